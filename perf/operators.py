@@ -241,8 +241,8 @@ def _plain(kind, case, s):
         return {"loss": loss, "dlogits": torch.where((scale != 0)[:, None], d, 0.0).to(logits.dtype)}
     valid, at, logp = _token_logp(z, total, tokens)
     if kind in ("score", "nll"):
-        # what the backward pass takes up again: the row's maximum and the sum; 0 and 1 where the token counts for nothing
-        saved = torch.stack([torch.where(valid, logits.amax(dim=1).float(), 0.0), torch.where(valid, total[:, 0], 1.0)])
+        # what the backward pass takes up again: the row's maximum and the sum; zeros where the token counts for nothing
+        saved = torch.stack([torch.where(valid, logits.amax(dim=1).float(), 0.0), torch.where(valid, total[:, 0], 0.0)])
     if kind == "score":
         return {"logp": logp, "saved": saved}
     if kind == "nll":
@@ -318,7 +318,7 @@ def exact(case, seed):
         top = s["logits"].max(dim=1).values.double()
         lse = torch.cat([torch.logsumexp(s["logits"][r:r + step].double() / tau, dim=1) for r in range(0, t, step)])
         found["logp"] = logp
-        found["saved"] = torch.stack([torch.where(valid, top, 0.0), torch.where(valid, torch.exp(lse - top / tau), 1.0)])
+        found["saved"] = torch.stack([torch.where(valid, top, 0.0), torch.where(valid, torch.exp(lse - top / tau), 0.0)])
         if kind == "score":
             return found
         total = (s["dlogp"].double() * torch.where(valid, lead, 0.0)).sum()
