@@ -9,7 +9,8 @@ Kinds (a case names one and gives its sizes; logits are [rows][vocab] of the cas
   distill     divergence from a teacher of whom the top K logits are kept, loss and gradient in one call
 
 Where `own` is false, run() computes the operators from elementary torch operations in 32 bits; where it is true, it calls the
-framework. Rows that do not count (a prompt's tokens, padding) have a token of -100 or a weight of 0.
+framework. Rows that do not count (a prompt's tokens, padding) have a token of -100 or a weight of 0. Gradients are the direction in
+which the loss falls, as every backward pass of the framework has them and its optimiser adds them.
 """
 import math
 
@@ -125,7 +126,7 @@ def prepare(case, seed):
         state["dlogits"] = torch.zeros(t, v, dtype=dtype, device="cuda")
     if kind in ("score", "nll"):
         tokens[out] = IGNORED
-        state["dlogp"] = -uniform(t) * _scale(case, t)
+        state["dlogp"] = uniform(t) * _scale(case, t)
     elif kind == "policy":
         state["mask"] = (~out).float()
         state["advantages"] = normal(t)
@@ -237,7 +238,7 @@ def _plain(kind, case, s):
         q, lnq = q / qt, e - qt.log()
         scale = s["mask"] * _scale(case, case["rows"])
         loss = scale * tau * tau * (q * (lnq - (z.gather(1, ids) - total.log()))).sum(dim=1)
-        d = (p * (scale * tau)[:, None]).scatter_add_(1, ids, q * (-scale * tau)[:, None])
+        d = (p * (-scale * tau)[:, None]).scatter_add_(1, ids, q * (scale * tau)[:, None])
         return {"loss": loss, "dlogits": torch.where((scale != 0)[:, None], d, 0.0).to(logits.dtype)}
     valid, at, logp = _token_logp(z, total, tokens)
     if kind in ("score", "nll"):
@@ -254,12 +255,12 @@ def _plain(kind, case, s):
         w = torch.where(on, s["mask"], 0.0) * _scale(case, case["rows"])
         ratio, a = (logp - s["old_logp"]).exp(), s["advantages"]
         free, held = ratio * a, ratio.clamp(1.0 - CLIP_LOW, 1.0 + CLIP_HIGH) * a
-        per_token, g = -torch.minimum(free, held), torch.where(free <= held, -free, 0.0)
+        per_token, g = -torch.minimum(free, held), torch.where(free <= held, free, 0.0)
         kl = torch.zeros_like(logp)
         if s["ref_logp"] is not None:
             d = s["ref_logp"] - logp
             kl = torch.where(on, d.expm1() - d, 0.0)
-            per_token, g = per_token + KL_COEF * kl, g - KL_COEF * d.expm1()
+            per_token, g = per_token + KL_COEF * kl, g + KL_COEF * d.expm1()
         g = torch.where(on, w * g, 0.0)
         return {"loss": torch.where(on, w * per_token, 0.0), "logp": logp, "kl": kl, "dlogits": _token_gradient(p, at, g, tau, logits.dtype)}
     # preference
@@ -278,7 +279,7 @@ def _plain(kind, case, s):
     else:
         up, down = 1.0 / (1.0 + (-BETA * h).exp()), 1.0 / (1.0 + (BETA * h).exp())
         loss, dh = -(1.0 - smooth) * up.log() - smooth * down.log(), BETA * (smooth * up - (1.0 - smooth) * down)
-    g = torch.cat([torch.stack([dh, -dh], dim=1).view(-1) * share[:2 * pairs] * scale, torch.zeros(1, dtype=torch.float64, device=h.device)])
+    g = torch.cat([torch.stack([-dh, dh], dim=1).view(-1) * share[:2 * pairs] * scale, torch.zeros(1, dtype=torch.float64, device=h.device)])
     g = torch.where(valid, g[seq].float(), 0.0)
     return {"loss": (loss * scale).float(), "rewards": (BETA * ratio).view(-1).float(), "dlogits": _token_gradient(p, at, g, tau, logits.dtype)}
 
@@ -307,7 +308,7 @@ def exact(case, seed):
             lnq = torch.log_softmax(s["teacher"][r:r + step].double() / tau, dim=1)
             lnp = x.gather(1, ids) / tau - torch.logsumexp(x / tau, dim=1, keepdim=True)
             loss = w * (lnq.exp() * (lnq - lnp)).sum(dim=1)
-            grads.append(torch.autograd.grad(loss.sum(), x)[0])
+            grads.append(torch.autograd.grad(-loss.sum(), x)[0])
             losses.append(loss.detach())
         return {"loss": torch.cat(losses), "dlogits": torch.cat(grads)}
     logp = torch.cat([_exact_logp(s["logits"][r:r + step], tokens[r:r + step].clamp(min=0), tau)[1] for r in range(0, t, step)])
@@ -349,7 +350,7 @@ def exact(case, seed):
                 losses.append((0.9 * torch.nn.functional.softplus(-m) + 0.1 * torch.nn.functional.softplus(m)) * _scale(case, case["pairs"]))
         total = torch.stack(losses).sum()
         found.update(loss=torch.stack(losses).detach(), rewards=torch.stack(rewards).detach())
-    g = torch.autograd.grad(total, lead)[0]
+    g = torch.autograd.grad(total if kind == "nll" else -total, lead)[0]
     grads = []
     for r in range(0, t, step):
         x = s["logits"][r:r + step].double().requires_grad_()
