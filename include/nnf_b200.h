@@ -448,6 +448,86 @@ NNF_API int nnf_cross_entropy_bwd(nnf_stream_t stream, float * dpredicted, const
 NNF_API int nnf_accuracy_fwd(nnf_stream_t stream, float * out, const float * predicted, const float * targets, const float * mask,
 	int top_n, int64_t n, int64_t c, int64_t hw);
 
+/* ---------------------------------------------------------------------------------------------
+ * Losses on the scores of a vocabulary: one row of logits for each token, the targets are indices. What the negative log likelihood
+ * above is for the classes of an image, these are for rows of 1e3 to 1e5 scores. No counterpart in the reference.
+ *
+ * Logits are a matrix of fp32, bf16 or fp16 rows that may be further apart than they are long (stride, in elements; any alignment),
+ * each of at most 1 MiB. Everything else is fp32 with one element for each row, except where stated. With tau = temperature:
+ *   M = max_j x_j,  S = sum_j exp((x_j - M)/tau),  p_j = exp((x_j - M)/tau)/S,  logp = (x_token - M)/tau - ln S
+ * in fp32; a gradient is rounded to the logits' type once, when it is stored (added: the sum is).
+ *
+ * A row counts for nothing where its token is outside [0, cols), its mask (a weight for each row, may be NULL: 1) is 0, or all its
+ * scores are -infinity. Such a row is not read (but in the last case): its loss, logp and kl are 0, its gradient is 0, whatever its
+ * scores hold. Elsewhere infinities and NaN take their course.
+ * As in every backward pass of this library, dlogits and dlogp are the direction in which the loss falls (its gradient negated: what
+ * nnf_apply_gradient adds, and what nnf_softmax_nll_bwd adds to when both end in one buffer).
+ * dlogits NULL: the loss alone. dlogits may be the logits themselves (same stride, not added to): each row's gradient takes its
+ * scores' place. add_to_destination accumulates into dlogits. The layers are losses: no output errors, `scale` and the mask weigh them. */
+typedef enum nnf_type
+{
+	NNF_F32 = 0,
+	NNF_BF16 = 1,
+	NNF_F16 = 2,
+	NNF_I32 = 3,
+	NNF_I64 = 4
+} nnf_type;
+
+typedef struct nnf_matrix
+{
+	void * data;          /* [rows][cols], a row every `stride` elements (stride >= cols); aligned to its element */
+	int32_t type;         /* nnf_type */
+	int64_t rows, cols, stride;
+} nnf_matrix;
+
+typedef struct nnf_indices
+{
+	const void * data;
+	int32_t type;         /* NNF_I32 or NNF_I64 */
+} nnf_indices;
+
+/* Log probabilities of one token of each row, and what reaches the logits of what has reached the log probabilities:
+ *   dlogits_j = dlogp/tau * ((j == token) - p_j)
+ * saved[2][rows] = {M, S} is what the backward pass takes up again (0, 0 where the row counts for nothing); NULL: not wanted.
+ * A row whose dlogp is 0 is not read. With dlogp = 1/rows this is the negative log likelihood of index targets. */
+NNF_API int nnf_token_logp_fwd(nnf_stream_t stream, float * logp, float * saved, const nnf_matrix * logits, const nnf_indices * tokens, float temperature);
+NNF_API int nnf_token_logp_bwd(nnf_stream_t stream, const nnf_matrix * dlogits, const float * dlogp, const nnf_matrix * logits, const nnf_indices * tokens,
+	const float * saved, float temperature, int add_to_destination);
+
+/* Clipped policy loss with a KL term, loss and gradient in one pass over the logits:
+ *   r = exp(logp - old_logp),  d = ref_logp - logp,  kl = exp(d) - 1 - d      (ref_logp NULL: no KL term, kl 0)
+ *   loss = scale*mask * ( -min(r*advantage, clip(r, 1 - clip_low, 1 + clip_high)*advantage) + kl_coef*kl )
+ *   dlogits_j = g/tau * ((j == token) - p_j),  g = scale*mask * ( (r*advantage where that is the minimum, else 0) + kl_coef*(exp(d) - 1) )
+ * kl (without scale, mask and coefficient) may be NULL. */
+NNF_API int nnf_policy_loss(nnf_stream_t stream, float * loss, float * logp, float * kl, const nnf_matrix * dlogits, const nnf_matrix * logits,
+	const nnf_indices * tokens, const float * old_logp, const float * advantages, const float * ref_logp, const float * mask,
+	float clip_low, float clip_high, float kl_coef, float temperature, float scale, int add_to_destination);
+
+/* Loss of paired sequences: the preferred one of pair i is rows offsets[2i] .. offsets[2i+1], the other one offsets[2i+1] .. offsets[2i+2]
+ * (2*pairs + 1 offsets that do not decrease, within [0, rows]). With s = sum of a sequence's log probabilities over the rows that count
+ * (average: their mean; 0 without any), q = s - ref_logp[sequence] and h = q[2i] - q[2i+1]:
+ *   NNF_PREFERENCE_LOGISTIC  loss = scale * ( (1 - label_smoothing)*ln(1 + exp(-beta*h)) + label_smoothing*ln(1 + exp(beta*h)) )
+ *   NNF_PREFERENCE_SQUARED   loss = scale * (h - 1/(2*beta))^2
+ *   rewards[sequence] = beta*q,  dlogp = -dloss/dlogp of each row,  dlogits as nnf_token_logp_bwd computes it from dlogp
+ * loss [pairs], ref_logp and rewards [2*pairs], logp, dlogp [rows], saved [2][rows]. Rows in front of the first sequence and behind the
+ * last one are left as they were in every output. Sums over a sequence are formed in fp64 in an order that its length alone decides. */
+typedef enum nnf_preference_kind
+{
+	NNF_PREFERENCE_LOGISTIC = 0,
+	NNF_PREFERENCE_SQUARED = 1
+} nnf_preference_kind;
+NNF_API int nnf_preference_loss(nnf_stream_t stream, float * loss, float * rewards, float * logp, float * saved, float * dlogp, const nnf_matrix * dlogits,
+	const nnf_matrix * logits, const nnf_indices * tokens, const nnf_indices * offsets, int64_t pairs, const float * ref_logp, int kind, float beta,
+	float label_smoothing, int average, float temperature, float scale, int add_to_destination);
+
+/* Distillation from a teacher of whom the top logits of each row are kept (teacher_ids, teacher_logits [rows][kept], kept <= 1024):
+ *   q = softmax(teacher_logits/tau) over the entries that are kept,  loss = scale*mask * tau^2 * sum_e q_e * (ln q_e - ln p_id(e))
+ *   dlogits_j = scale*mask * tau * (sum of q_e over the entries with id(e) = j, less p_j)
+ * An entry whose id is outside [0, cols) or whose logit is -infinity is not kept; a row without entries counts for nothing. An id that
+ * is there twice holds the mass of both. loss and dlogits without any rounding in between, in one pass over the logits. */
+NNF_API int nnf_distill_topk_loss(nnf_stream_t stream, float * loss, const nnf_matrix * dlogits, const nnf_matrix * logits, const nnf_matrix * teacher_ids,
+	const nnf_matrix * teacher_logits, const float * mask, float temperature, float scale, int add_to_destination);
+
 /* Batch-sharded training batch norm in ONE launch per direction and GPU (the sharded form of
  * nnf_bn_train_fwd / nnf_bn_train_bwd): statistics and apply work items share the launch, the second read
  * of x (and dy) comes from L2, and the per-channel sums cross the GPUs inside the launch - the item that

@@ -46,6 +46,14 @@ class Pool(ct.Structure):
                 ("round_up_w", ct.c_int32), ("round_up_h", ct.c_int32), ("is_min", ct.c_int32)]
 
 
+class Matrix(ct.Structure):
+    _fields_ = [("data", ct.c_void_p), ("type", ct.c_int32), ("rows", ct.c_int64), ("cols", ct.c_int64), ("stride", ct.c_int64)]
+
+
+class Indices(ct.Structure):
+    _fields_ = [("data", ct.c_void_p), ("type", ct.c_int32)]
+
+
 _native.set_types(NnfError, Act, Pool)
 
 
@@ -57,7 +65,10 @@ class OptPart(ct.Structure):
 
 MOMENTUM_NONE, MOMENTUM_VANILLA, MOMENTUM_NESTEROV, MOMENTUM_ADAM = range(4)
 
+PREFERENCE_LOGISTIC, PREFERENCE_SQUARED = range(2)
+
 _ACTP, _POOLP = ct.POINTER(Act), ct.POINTER(Pool)
+_MATP, _IDXP = ct.POINTER(Matrix), ct.POINTER(Indices)
 
 class RunningConfiguration(ct.Structure):
     _fields_ = [(name, ct.c_int32) for name in (
@@ -114,6 +125,11 @@ _SIGNATURES = {
     "nnf_cross_entropy_bwd": (_I, [_P, _P, _P, _P, _P, _F, _I64, _I64, _I64, _I]),
     "nnf_softmax_nll_fwd": (_I, [_P, _P, _P, _P, _P, _P, _F, _I64, _I64, _I64]),
     "nnf_softmax_nll_bwd": (_I, [_P, _P, _P, _P, _P, _F, _I64, _I64, _I64, _I]),
+    "nnf_token_logp_fwd": (_I, [_P, _P, _P, _MATP, _IDXP, _F]),
+    "nnf_token_logp_bwd": (_I, [_P, _MATP, _P, _MATP, _IDXP, _P, _F, _I]),
+    "nnf_policy_loss": (_I, [_P, _P, _P, _P, _MATP, _MATP, _IDXP, _P, _P, _P, _P, _F, _F, _F, _F, _F, _I]),
+    "nnf_preference_loss": (_I, [_P, _P, _P, _P, _P, _P, _MATP, _MATP, _IDXP, _IDXP, _I64, _P, _I, _F, _F, _I, _F, _F, _I]),
+    "nnf_distill_topk_loss": (_I, [_P, _P, _MATP, _MATP, _MATP, _MATP, _P, _F, _F, _I]),
     "nnf_bn_train_mailbox_bytes": (_SZ, [_I64]),
     "nnf_bn_train_sharded_supported": (_I, [_I64, _I64, _I64]),
     "nnf_bn_train_fwd_sharded": (_I, [_P, _P, _P, _P, _P, _P, _P, _F, _ACTP, _I, _I64, _I64, _I64, _D, _P, _SZ, ct.POINTER(_P), _I, _I, ct.c_uint32]),
@@ -407,6 +423,44 @@ def softmax_nll_fwd(probs, err, logits, targets, mask=None, scale=1.0, stream=No
 
 def softmax_nll_bwd(dlogits, probs, targets, mask=None, scale=1.0, add_to_destination=False, stream=None):
     _native.softmax_nll_bwd(dlogits, probs, targets, mask, scale, add_to_destination, stream)
+
+
+# Losses on the scores of a vocabulary. Logits [rows][vocabulary] are fp32, bf16 or fp16, contiguous within a row (rows may be further
+# apart); tokens, teacher_ids and offsets are int32 or int64; everything else is fp32 with one element for each row, unless stated.
+# A row whose token lies outside the vocabulary (-100, say), whose mask is 0 or whose scores are all -infinity counts for nothing:
+# loss, log probability and gradient are 0. dlogits may be the logits themselves; as everywhere in the library it is the direction in which
+# the loss falls, what apply_gradient adds.
+
+
+def token_logp_fwd(logp, saved, logits, tokens, temperature=1.0, stream=None):
+    """Log probability of each row's token under softmax(logits / temperature). saved [2][rows] (or None) is for token_logp_bwd."""
+    _native.token_logp_fwd(logp, saved, logits, tokens, temperature, stream)
+
+
+def token_logp_bwd(dlogits, dlogp, logits, tokens, saved, temperature=1.0, add_to_destination=False, stream=None):
+    _native.token_logp_bwd(dlogits, dlogp, logits, tokens, saved, temperature, add_to_destination, stream)
+
+
+def policy_loss(loss, logp, logits, tokens, old_logp, advantages, ref_logp=None, mask=None, kl=None, dlogits=None, clip_low=0.2, clip_high=0.2,
+                kl_coef=0.0, temperature=1.0, scale=1.0, add_to_destination=False, stream=None):
+    """Clipped policy loss with a KL term towards ref_logp (None: without), and its gradient (dlogits None: the loss alone)."""
+    _native.policy_loss(loss, logp, kl, dlogits, logits, tokens, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coef, temperature,
+                        scale, add_to_destination, stream)
+
+
+def preference_loss(loss, rewards, logp, saved, dlogp, logits, tokens, offsets, ref_logp, dlogits=None, kind=PREFERENCE_LOGISTIC, beta=0.1,
+                    label_smoothing=0.0, average=False, temperature=1.0, scale=1.0, add_to_destination=False, stream=None):
+    """Loss of the pairs (preferred sequence, other one) that `offsets` [2 * pairs + 1] cuts the rows into, and its gradient. loss [pairs];
+    ref_logp, rewards [2 * pairs]; logp, dlogp [rows] and saved [2][rows] are written too. Rows outside the sequences stay as they were."""
+    _native.preference_loss(loss, rewards, logp, saved, dlogp, dlogits, logits, tokens, offsets, ref_logp, kind, beta, label_smoothing, average,
+                            temperature, scale, add_to_destination, stream)
+
+
+def distill_topk_loss(loss, logits, teacher_ids, teacher_logits, mask=None, dlogits=None, temperature=1.0, scale=1.0, add_to_destination=False,
+                      stream=None):
+    """Divergence of softmax(logits / temperature) from a teacher of whom teacher_logits [rows][kept] at teacher_ids are known, and its
+    gradient. An id outside the vocabulary is no entry."""
+    _native.distill_topk_loss(loss, dlogits, logits, teacher_ids, teacher_logits, mask, temperature, scale, add_to_destination, stream)
 
 
 def bn_train_sharded_supported(n, c, hw):

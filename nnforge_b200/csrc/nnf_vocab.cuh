@@ -1,0 +1,202 @@
+// What the losses on the scores of a vocabulary (nnf_vocab_loss.cu) share: rows of fp32, bf16 or fp16 that start and end anywhere,
+// the running maximum and sum of a softmax, and their exchange across a thread-block cluster.
+#pragma once
+
+#include "nnf_common.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace nnf
+{
+	// The elements of 16 bytes, as floats and back. Rounding to 16 bits happens once, to nearest, when a gradient is stored.
+	template <class T> struct piece;
+
+	template <> struct piece<float>
+	{
+		static constexpr int N = 4;
+		static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[N])
+		{
+			f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+		}
+		static __device__ __forceinline__ uint4 pack(const float (&f)[N])
+		{
+			return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+		}
+		static __device__ __forceinline__ uint32_t bits(const float * p) { return __float_as_uint(*p); }
+		static __device__ __forceinline__ float value(const float * p) { return *p; }
+		static __device__ __forceinline__ void store(float * p, float v) { *p = v; }
+		static constexpr uint32_t kNothing = 0xff800000u;   // -infinity, in every element of the word
+	};
+
+	template <> struct piece<__nv_bfloat16>
+	{
+		static constexpr int N = 8;
+		static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[N])
+		{
+			const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+			#pragma unroll
+			for (int i = 0; i < 4; ++i)
+			{
+				f[2 * i] = __uint_as_float(w[i] << 16);
+				f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+			}
+		}
+		static __device__ __forceinline__ uint4 pack(const float (&f)[N])
+		{
+			uint32_t w[4];
+			#pragma unroll
+			for (int i = 0; i < 4; ++i)
+			{
+				const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+				w[i] = *reinterpret_cast<const uint32_t *>(&h);
+			}
+			return make_uint4(w[0], w[1], w[2], w[3]);
+		}
+		static __device__ __forceinline__ uint32_t bits(const __nv_bfloat16 * p) { return __bfloat16_as_ushort(*p); }
+		static __device__ __forceinline__ float value(const __nv_bfloat16 * p) { return __bfloat162float(*p); }
+		static __device__ __forceinline__ void store(__nv_bfloat16 * p, float v) { *p = __float2bfloat16_rn(v); }
+		static constexpr uint32_t kNothing = 0xff80ff80u;
+	};
+
+	template <> struct piece<__half>
+	{
+		static constexpr int N = 8;
+		static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[N])
+		{
+			const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+			#pragma unroll
+			for (int i = 0; i < 4; ++i)
+			{
+				const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+				f[2 * i] = t.x;
+				f[2 * i + 1] = t.y;
+			}
+		}
+		static __device__ __forceinline__ uint4 pack(const float (&f)[N])
+		{
+			uint32_t w[4];
+			#pragma unroll
+			for (int i = 0; i < 4; ++i)
+			{
+				const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+				w[i] = *reinterpret_cast<const uint32_t *>(&h);
+			}
+			return make_uint4(w[0], w[1], w[2], w[3]);
+		}
+		static __device__ __forceinline__ uint32_t bits(const __half * p) { return __half_as_ushort(*p); }
+		static __device__ __forceinline__ float value(const __half * p) { return __half2float(*p); }
+		static __device__ __forceinline__ void store(__half * p, float v) { *p = __float2half_rn(v); }
+		static constexpr uint32_t kNothing = 0xfc00fc00u;
+	};
+
+	// The 16-byte frame of a row of `cols` elements that starts anywhere: every aligned piece that holds one of its elements. Only the
+	// first and the last piece can be partial; their elements are read and written one by one, the neighbouring rows' stay untouched.
+	template <class T>
+	struct row_frame
+	{
+		static constexpr int N = piece<T>::N;
+		T * at;            // the row's first element
+		int shift;         // elements of the first piece in front of it
+		int pieces;
+		int cols;
+
+		__device__ __forceinline__ row_frame(T * row, int cols) : at(row), cols(cols)
+		{
+			shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+			pieces = (shift + cols + N - 1) / N;
+		}
+		__device__ __forceinline__ bool whole(int i) const { return (i > 0 || shift == 0) && (i + 1) * N - shift <= cols; }
+		__device__ __forceinline__ uint4 * address(int i) const { return reinterpret_cast<uint4 *>(at - shift) + i; }
+		__device__ __forceinline__ bool has(int i, int k) const { const int e = i * N - shift + k; return e >= 0 && e < cols; }
+
+		// elements outside the row: -infinity
+		__device__ __forceinline__ uint4 load(int i) const
+		{
+			if (whole(i))
+				return __ldcs(address(i));
+			uint32_t w[4];
+			#pragma unroll
+			for (int k = 0; k < 4; ++k)
+			{
+				w[k] = piece<T>::kNothing;
+				if (N == 4)
+				{
+					if (has(i, k))
+						w[k] = piece<T>::bits(at + i * N - shift + k);
+				}
+				else
+				{
+					if (has(i, 2 * k))
+						w[k] = (w[k] & 0xffff0000u) | piece<T>::bits(at + i * N - shift + 2 * k);
+					if (has(i, 2 * k + 1))
+						w[k] = (w[k] & 0xffffu) | (piece<T>::bits(at + i * N - shift + 2 * k + 1) << 16);
+				}
+			}
+			return make_uint4(w[0], w[1], w[2], w[3]);
+		}
+	};
+
+	// maximum and sum of exp2((x - maximum) * k) of some elements; nothing: (-infinity, 0)
+	struct softmax_part
+	{
+		float m, s;
+	};
+
+	__device__ __forceinline__ float exp2_of(float x)
+	{
+		float e;
+		asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
+		return e;
+	}
+
+	// What a part's exponentials are multiplied with when the maximum becomes m. A part without a maximum (-infinity) keeps its sum: 0, or
+	// NaN where an element was NaN, which no maximum shows.
+	__device__ __forceinline__ float rescale(float part_m, float m, float k)
+	{
+		return part_m == m ? 1.0F : exp2_of((part_m - m) * k);
+	}
+
+	__device__ __forceinline__ softmax_part join(const softmax_part& a, const softmax_part& b, float k)
+	{
+		softmax_part r;
+		r.m = fmaxf(a.m, b.m);
+		r.s = a.s * rescale(a.m, r.m, k) + b.s * rescale(b.m, r.m, k);
+		return r;
+	}
+
+	__device__ __forceinline__ float vocab_warp_max(float v)
+	{
+		#pragma unroll
+		for (int o = 16; o > 0; o >>= 1)
+			v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+		return v;
+	}
+
+	__device__ __forceinline__ float vocab_warp_sum(float v)
+	{
+		#pragma unroll
+		for (int o = 16; o > 0; o >>= 1)
+			v += __shfl_xor_sync(0xffffffffu, v, o);
+		return v;
+	}
+
+	// ---- thread-block clusters -----------------------------------------------------------------------
+	__device__ __forceinline__ uint32_t vocab_cluster_rank()
+	{
+		uint32_t r;
+		asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+		return r;
+	}
+
+	__device__ __forceinline__ void vocab_cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+	__device__ __forceinline__ void vocab_cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+	// a store into the shared memory of another CTA of the cluster, at the address that `p` has in this one
+	__device__ __forceinline__ void vocab_cluster_store(const softmax_part * p, uint32_t rank, softmax_part v)
+	{
+		uint32_t a;
+		asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+		asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" :: "r"(a), "f"(v.m), "f"(v.s) : "memory");
+	}
+}

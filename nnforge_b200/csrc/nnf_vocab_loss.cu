@@ -1,0 +1,916 @@
+// Losses on the scores of a vocabulary: log probabilities of given tokens (forward and backward), the clipped policy loss with a KL
+// term, the loss of paired sequences, and distillation from a teacher's top logits. Logits are rows of fp32, bf16 or fp16, one for each
+// token, and the targets are indices: what softmax + negative log likelihood (nnf_loss.cu) is for the classes of an image, with dense
+// targets and stored probabilities, these are where a row has 1e3..1e5 scores.
+//
+//   M = max_j x_j,  S = sum_j exp((x_j - M)/tau),  p_j = exp((x_j - M)/tau)/S,  logp = (x_a - M)/tau - ln S
+//   every gradient is  dx_j = (what the targets hold at j) - c*p_j,  c one number for the row: the direction in which the loss falls,
+//   as the library's backward passes have it and its optimiser step adds it.
+//
+// All are bound by HBM: a row is read once, kept in registers while its maximum and sum are found (one exchange: a warp's maximum and
+// sum against it, joined by all warps), and its gradient written from there. A row that does not fit one CTA's registers, or that
+// would leave SMs idle because there are few rows, is split over a thread-block cluster, whose CTAs exchange their parts through
+// distributed shared memory. Maximum, sum and everything behind them are fp32; a gradient is rounded once, when it is stored.
+#include "nnf_vocab.cuh"
+
+namespace nnf
+{
+	namespace
+	{
+		constexpr int kVocabPieces = 8;          // 16-byte pieces of a row that a thread holds
+		constexpr int kVocabThreads = 1024;      // most threads of a CTA
+		constexpr int kVocabCluster = 8;         // most CTAs of a row (the portable cluster size)
+		constexpr int kVocabWarps = kVocabThreads / 32;
+		constexpr int kMaxKept = 1024;           // most logits that are kept of a teacher's row
+
+		enum { kScore = 0, kPolicy = 1, kDistill = 2 };
+
+		struct vocab_params
+		{
+			const void * x;
+			void * dx;                 // gradient, or null
+			int64_t ldx, lddx;
+			int64_t rows;
+			int cols;
+			int add;                   // the gradient is added to what dx holds
+			float tau, inv_tau, k;     // k = log2(e)/tau
+			int cluster;               // CTAs of a row
+			// targets
+			const void * tokens;
+			int tokens_wide;           // 64-bit indices
+			const float * mask;
+			float scale;
+			float * loss;
+			float * logp;
+			float * saved;             // [2][rows]: M, S
+			// score: only the rows in [offsets[0], offsets[sequences]) are written, or null
+			const void * offsets;
+			int offsets_wide;
+			int64_t sequences;
+			// policy
+			const float * old_logp, * advantages, * ref_logp;
+			float * kl;
+			float low, high, kl_coef;
+			// distillation
+			const void * ids, * teacher;
+			int64_t ld_ids, ld_teacher;
+			int ids_wide, teacher_type, kept;
+		};
+
+		__device__ __forceinline__ int64_t index_at(const void * p, int wide, int64_t i)
+		{
+			return wide ? __ldg(static_cast<const long long *>(p) + i) : (int64_t)__ldg(static_cast<const int *>(p) + i);
+		}
+
+		__device__ __forceinline__ float value_at(const void * p, int type, int64_t i)
+		{
+			if (type == NNF_BF16)
+				return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+			if (type == NNF_F16)
+				return __half2float(static_cast<const __half *>(p)[i]);
+			return __ldg(static_cast<const float *>(p) + i);
+		}
+
+		// the rows that the packed sequences cover
+		__device__ __forceinline__ void covered_rows(const vocab_params& p, int64_t& begin, int64_t& end)
+		{
+			begin = index_at(p.offsets, p.offsets_wide, 0);
+			end = index_at(p.offsets, p.offsets_wide, p.sequences);
+			begin = begin < 0 ? 0 : begin;
+			end = end > p.rows ? p.rows : end;
+		}
+
+		// stores a piece of the gradient's row: whole and aligned pieces at once, others element by element
+		template <class T, class F>
+		__device__ __forceinline__ void store_piece(const row_frame<T>& x, T * dx, bool aligned, int i, int add, F f)
+		{
+			constexpr int N = piece<T>::N;
+			const int first = i * N - x.shift;
+			if (aligned && x.whole(i))
+			{
+				uint4 * to = reinterpret_cast<uint4 *>(dx + first);
+				float g[N];
+				if (add)
+				{
+					piece<T>::unpack(*to, g);
+					#pragma unroll
+					for (int e = 0; e < N; ++e)
+						g[e] += f(e);
+				}
+				else
+				{
+					#pragma unroll
+					for (int e = 0; e < N; ++e)
+						g[e] = f(e);
+				}
+				__stcs(to, piece<T>::pack(g));
+			}
+			else
+			{
+				#pragma unroll
+				for (int e = 0; e < N; ++e)
+					if (x.has(i, e))
+						piece<T>::store(dx + first + e, add ? piece<T>::value(dx + first + e) + f(e) : f(e));
+			}
+		}
+
+		struct distill_shared
+		{
+			int * id;         // -1: the entry does not count
+			float * q;        // the teacher's probability
+			float * lnq;
+			float * x;        // the student's score
+			float * old;      // what the gradient held (it is added to)
+			uint32_t * seen;  // a bit for each of this CTA's columns
+		};
+
+		// NP: pieces of a thread
+		template <class T, int OP, int NP>
+		__global__ void __launch_bounds__(kVocabThreads) vocab_rows_kernel(const vocab_params p)
+		{
+			constexpr int N = piece<T>::N;
+			extern __shared__ __align__(16) unsigned char s_dyn[];
+			__shared__ softmax_part s_part[2][kVocabCluster * kVocabWarps];
+			pdl_begin();
+
+			const uint32_t split = (uint32_t)p.cluster;
+			const uint32_t rank = split > 1 ? vocab_cluster_rank() : 0;
+			const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+			const int parts = (int)split * warps;
+			const int64_t row_step = gridDim.x / split;
+			if (split > 1)
+			{
+				vocab_cluster_arrive();   // every CTA of the cluster has started before the first store into another one
+				vocab_cluster_wait();
+			}
+			distill_shared d = {};
+			if (OP == kDistill)
+			{
+				d.id = reinterpret_cast<int *>(s_dyn);
+				d.q = reinterpret_cast<float *>(d.id + p.kept);
+				d.lnq = d.q + p.kept;
+				d.x = d.lnq + p.kept;
+				d.old = d.x + p.kept;
+				d.seen = reinterpret_cast<uint32_t *>(d.old + p.kept);
+				const int words = (NP * (int)blockDim.x * N + 31) / 32;
+				for (int i = threadIdx.x; i < words; i += blockDim.x)
+					d.seen[i] = 0;
+			}
+			int64_t begin = 0, end = p.rows;
+			if (OP == kScore && p.offsets)
+				covered_rows(p, begin, end);
+
+			int phase = 0;
+			for (int64_t row = begin + blockIdx.x / split; row < end; row += row_step)
+			{
+				const row_frame<T> x(const_cast<T *>(static_cast<const T *>(p.x)) + row * p.ldx, p.cols);
+				T * const dx = p.dx ? static_cast<T *>(p.dx) + row * p.lddx : nullptr;
+				const bool aligned = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x.at)) & 15) == 0;
+				const int per = (x.pieces + (int)split - 1) / (int)split;
+				const int from = (int)rank * per, to = min(from + per, x.pieces);   // this CTA's pieces
+
+				const float w = OP != kScore && p.mask ? __ldg(p.mask + row) : 1.0F;
+				int64_t token = 0;
+				bool on = w != 0.0F;
+				if (OP != kDistill)
+				{
+					token = index_at(p.tokens, p.tokens_wide, row);
+					on = on && token >= 0 && token < p.cols;
+				}
+				softmax_part total = {0.0F, 0.0F};
+				float xa = 0.0F;
+				uint4 v[NP];
+				bool any = false;
+				if (on)
+				{
+					#pragma unroll
+					for (int j = 0; j < NP; ++j)
+					{
+						const int i = from + j * (int)blockDim.x + (int)threadIdx.x;
+						v[j] = make_uint4(piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing);
+						if (i < to)
+							v[j] = x.load(i);
+					}
+					if (OP != kDistill)
+						xa = piece<T>::value(x.at + token);
+					else if (warp == 0)
+					{
+						// the teacher's probabilities over the logits that are kept: one warp, while the row is on its way
+						float m = -INFINITY;
+						for (int e = lane; e < p.kept; e += 32)
+						{
+							const int64_t id = index_at(p.ids, p.ids_wide, row * p.ld_ids + e);
+							const bool in = id >= 0 && id < p.cols;
+							const float t = in ? value_at(p.teacher, p.teacher_type, row * p.ld_teacher + e) : -INFINITY;
+							const int i = in ? (int)(id + x.shift) / N : -1;
+							d.id[e] = in ? (int)id : -1;
+							d.lnq[e] = t;
+							d.x[e] = in && (rank == 0 || (i >= from && i < to)) ? piece<T>::value(x.at + id) : 0.0F;
+							if (p.add && i >= from && i < to)
+								d.old[e] = piece<T>::value(dx + id);
+							m = fmaxf(m, t);
+						}
+						m = vocab_warp_max(m);
+						const float base = m == -INFINITY ? 0.0F : m;
+						float s = 0.0F;
+						for (int e = lane; e < p.kept; e += 32)
+							s += d.q[e] = expf((d.lnq[e] - base) * p.inv_tau);
+						s = vocab_warp_sum(s);
+						const float r = 1.0F / s, ln = logf(s);
+						for (int e = lane; e < p.kept; e += 32)
+						{
+							d.q[e] = s == 0.0F ? 0.0F : d.q[e] * r;
+							d.lnq[e] = (d.lnq[e] - base) * p.inv_tau - ln;
+						}
+						any = s != 0.0F;
+					}
+
+					float m = -INFINITY;
+					#pragma unroll
+					for (int j = 0; j < NP; ++j)
+					{
+						float f[N];
+						piece<T>::unpack(v[j], f);
+						#pragma unroll
+						for (int e = 0; e < N; ++e)
+							m = fmaxf(m, f[e]);
+					}
+					softmax_part part;
+					part.m = vocab_warp_max(m);
+					const float base = part.m == -INFINITY ? 0.0F : part.m;
+					part.s = 0.0F;
+					#pragma unroll
+					for (int j = 0; j < NP; ++j)
+					{
+						float f[N];
+						piece<T>::unpack(v[j], f);
+						#pragma unroll
+						for (int e = 0; e < N; ++e)
+							part.s += exp2_of((f[e] - base) * p.k);
+					}
+					part.s = vocab_warp_sum(part.s);
+
+					// every warp gets every warp's part, those of the cluster's other CTAs included
+					softmax_part * const slots = s_part[phase];
+					phase ^= 1;   // a slot is written again two exchanges later: one barrier in between is enough
+					if (split > 1)
+					{
+						if (lane < (int)split)
+							vocab_cluster_store(slots + rank * warps + warp, lane, part);
+						vocab_cluster_arrive();
+						vocab_cluster_wait();
+					}
+					else
+					{
+						if (lane == 0)
+							slots[warp] = part;
+						__syncthreads();
+					}
+					total.m = -INFINITY;
+					for (int i = lane; i < parts; i += 32)
+						total.m = fmaxf(total.m, slots[i].m);
+					total.m = vocab_warp_max(total.m);
+					for (int i = lane; i < parts; i += 32)
+						total.s += slots[i].s * rescale(slots[i].m, total.m, p.k);
+					total.s = vocab_warp_sum(total.s);
+					on = total.s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
+				}
+
+				// the row's loss, and what its probabilities are multiplied with
+				float c = 0.0F, at_token = 0.0F;
+				const bool first = rank == 0 && threadIdx.x == 0;
+				if (OP == kScore)
+				{
+					if (first)
+					{
+						p.logp[row] = on ? (xa - total.m) * p.inv_tau - logf(total.s) : 0.0F;
+						if (p.saved)
+						{
+							p.saved[row] = on ? total.m : 0.0F;
+							p.saved[p.rows + row] = on ? total.s : 0.0F;
+						}
+					}
+					continue;
+				}
+				const float weight = p.scale * w;
+				if (OP == kPolicy)
+				{
+					float logp = 0.0F, kl = 0.0F, loss = 0.0F;
+					if (on)
+					{
+						logp = (xa - total.m) * p.inv_tau - logf(total.s);
+						const float a = __ldg(p.advantages + row), ratio = expf(logp - __ldg(p.old_logp + row));
+						const float free = ratio * a, held = fminf(fmaxf(ratio, p.low), p.high) * a;
+						// min() that keeps a NaN
+						loss = -(free <= held ? free : held < free ? held : free + held);
+						float g = held < free ? 0.0F : free;
+						if (p.ref_logp)
+						{
+							const float gap = __ldg(p.ref_logp + row) - logp, grown = expm1f(gap);
+							kl = grown - gap;
+							loss += p.kl_coef * kl;
+							g += p.kl_coef * grown;
+						}
+						g = weight != 0.0F ? g * weight * p.inv_tau : 0.0F;
+						loss = weight != 0.0F ? loss * weight : 0.0F;
+						c = -g / total.s;
+						at_token = -g * expm1f(logp);   // g * (1 - p)
+					}
+					if (first)
+					{
+						p.loss[row] = loss;
+						p.logp[row] = logp;
+						if (p.kl)
+							p.kl[row] = kl;
+					}
+					on = on && at_token != 0.0F | c != 0.0F;
+				}
+				if (OP == kDistill)
+				{
+					// the teacher's row is known to the first warp
+					if (rank == 0 && warp == 0)
+					{
+						float sum = 0.0F;
+						if (on && any && weight != 0.0F)
+						{
+							const float ln = logf(total.s);
+							for (int e = lane; e < p.kept; e += 32)
+								if (d.q[e] != 0.0F)
+									sum += d.q[e] * (d.lnq[e] - ((d.x[e] - total.m) * p.inv_tau - ln));
+							sum = vocab_warp_sum(sum) * (weight * p.tau * p.tau);
+						}
+						if (lane == 0)
+							p.loss[row] = sum;
+					}
+				}
+				if (!dx)
+				{
+					if (OP == kDistill)
+						__syncthreads();   // the teacher's row is read before the next one takes its place
+					continue;
+				}
+				if (OP == kDistill)
+				{
+					const bool valid = __syncthreads_or(any);
+					on = on && valid && weight != 0.0F;
+					c = on ? -weight * p.tau / total.s : 0.0F;
+				}
+				if (!on)
+				{
+					if (!p.add)
+						for (int i = from + (int)threadIdx.x; i < to; i += blockDim.x)
+							store_piece<T>(x, dx, aligned, i, 0, [](int) { return 0.0F; });
+					continue;
+				}
+				const int token_piece = OP == kPolicy ? (int)(token + x.shift) / N : -1, token_place = (int)(token + x.shift) % N;
+				#pragma unroll
+				for (int j = 0; j < NP; ++j)
+				{
+					const int i = from + j * (int)blockDim.x + (int)threadIdx.x;
+					if (i < to)
+					{
+						float f[N];
+						piece<T>::unpack(v[j], f);
+						#pragma unroll
+						for (int e = 0; e < N; ++e)
+							f[e] = exp2_of((f[e] - total.m) * p.k) * c;
+						if (OP == kPolicy && i == token_piece)
+						{
+							#pragma unroll
+							for (int e = 0; e < N; ++e)
+								f[e] = e == token_place ? at_token : f[e];
+						}
+						store_piece<T>(x, dx, aligned, i, p.add, [&](int e) { return f[e]; });
+					}
+				}
+				if (OP == kDistill)
+				{
+					// The columns that the teacher kept: c*(q - p), written over -c*p. An index that is there twice holds the sum of both; the
+					// first of its entries writes it. `seen` shows whether there is one at all.
+					bool twice = false;
+					for (int e = threadIdx.x; e < p.kept; e += blockDim.x)
+					{
+						const int col = d.id[e] < 0 ? -1 : d.id[e] + x.shift - from * N;
+						if (d.id[e] >= 0 && col >= 0 && col < (to - from) * N)
+						{
+							const uint32_t bit = 1u << (col & 31);
+							twice = twice || (atomicOr(d.seen + (col >> 5), bit) & bit);
+						}
+					}
+					twice = __syncthreads_or(twice);   // also: the pieces above are written
+					const float share = weight * p.tau;
+					for (int e = threadIdx.x; e < p.kept; e += blockDim.x)
+					{
+						const int id = d.id[e], col = id < 0 ? -1 : id + x.shift - from * N;
+						if (id >= 0 && col >= 0 && col < (to - from) * N)
+						{
+							d.seen[col >> 5] = 0;
+							float q = d.q[e];
+							bool leads = true;
+							if (twice)
+							{
+								q = 0.0F;
+								for (int o = 0; o < p.kept; ++o)
+									if (d.id[o] == id)
+									{
+										leads = leads && o >= e;
+										q += d.q[o];
+									}
+							}
+							if (leads)
+							{
+								const float g = exp2_of((d.x[e] - total.m) * p.k) * c + share * q;
+								piece<T>::store(dx + id, p.add ? d.old[e] + g : g);
+							}
+						}
+					}
+					__syncthreads();
+				}
+			}
+		}
+
+		// ---- backward of the log probabilities: one pass, nothing to be found first ------------------------
+		struct vocab_bwd_params
+		{
+			const void * x;
+			void * dx;
+			int64_t ldx, lddx;
+			int64_t rows;
+			int cols;
+			int add;
+			float inv_tau, k;
+			const void * tokens;
+			int tokens_wide;
+			const float * dlogp, * saved;
+			const void * offsets;      // as for the score, or null
+			int offsets_wide;
+			int64_t sequences;
+			int slices;                // CTAs of a row
+		};
+
+		constexpr int kBwdThreads = 256, kBwdPieces = 4;
+
+		template <class T>
+		__global__ void __launch_bounds__(kBwdThreads) vocab_bwd_kernel(const vocab_bwd_params p)
+		{
+			constexpr int N = piece<T>::N;
+			pdl_begin();
+			const int64_t row = blockIdx.x / p.slices;
+			if (p.offsets)
+			{
+				vocab_params q = {};
+				q.offsets = p.offsets; q.offsets_wide = p.offsets_wide; q.sequences = p.sequences; q.rows = p.rows;
+				int64_t begin, end;
+				covered_rows(q, begin, end);
+				if (row < begin || row >= end)
+					return;
+			}
+			const row_frame<T> x(const_cast<T *>(static_cast<const T *>(p.x)) + row * p.ldx, p.cols);
+			T * const dx = static_cast<T *>(p.dx) + row * p.lddx;
+			const bool aligned = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x.at)) & 15) == 0;
+			const int64_t token = index_at(p.tokens, p.tokens_wide, row);
+			const float g = __ldg(p.dlogp + row) * p.inv_tau, m = __ldg(p.saved + row), s = __ldg(p.saved + p.rows + row);
+			const bool on = token >= 0 && token < p.cols && s != 0.0F && g != 0.0F;
+			const int from = (int)(blockIdx.x % p.slices) * (int)(blockDim.x * kBwdPieces) + (int)threadIdx.x;
+			if (!on)
+			{
+				if (!p.add)
+					for (int j = 0, i = from; j < kBwdPieces && i < x.pieces; ++j, i += blockDim.x)
+						store_piece<T>(x, dx, aligned, i, 0, [](int) { return 0.0F; });
+				return;
+			}
+			const float c = -g / s;
+			const int token_piece = (int)(token + x.shift) / N, token_place = (int)(token + x.shift) % N;
+			uint4 v[kBwdPieces];
+			#pragma unroll
+			for (int j = 0; j < kBwdPieces; ++j)
+				if (from + j * (int)blockDim.x < x.pieces)
+					v[j] = x.load(from + j * (int)blockDim.x);
+			#pragma unroll
+			for (int j = 0; j < kBwdPieces; ++j)
+			{
+				const int i = from + j * (int)blockDim.x;
+				if (i < x.pieces)
+				{
+					float f[N];
+					piece<T>::unpack(v[j], f);
+					float at_token = 0.0F;
+					if (i == token_piece)
+					{
+						#pragma unroll
+						for (int e = 0; e < N; ++e)
+							at_token = e == token_place ? f[e] : at_token;
+						at_token = -g * expm1f((at_token - m) * p.inv_tau - logf(s));   // g * (1 - p)
+					}
+					#pragma unroll
+					for (int e = 0; e < N; ++e)
+					{
+						f[e] = exp2_of((f[e] - m) * p.k) * c;
+						if (i == token_piece && e == token_place)
+							f[e] = at_token;
+					}
+					store_piece<T>(x, dx, aligned, i, p.add, [&](int e) { return f[e]; });
+				}
+			}
+		}
+
+		// ---- pairs of sequences: sums of their log probabilities, the loss, and its gradient for every token ----
+		struct pair_params
+		{
+			const float * logp, * saved, * ref_logp;
+			const void * offsets;
+			int offsets_wide;
+			int64_t rows;
+			float * loss, * rewards, * dlogp;
+			float beta, smoothing, scale;
+			int kind, average;
+		};
+
+		constexpr int kPairThreads = 256;
+
+		__device__ __forceinline__ float softplus(float x)
+		{
+			return fmaxf(x, 0.0F) + log1pf(expf(-fabsf(x)));
+		}
+
+		// a CTA per pair; sums in double, in an order that depends on nothing but the lengths
+		__global__ void __launch_bounds__(kPairThreads) vocab_pair_kernel(const pair_params p)
+		{
+			__shared__ double s_sum[2][kPairThreads / 32];
+			__shared__ long long s_count[2][kPairThreads / 32];
+			pdl_begin();
+			const int64_t pair = blockIdx.x;
+			int64_t begin[2], end[2];
+			double sum[2];
+			long long count[2];
+			#pragma unroll
+			for (int side = 0; side < 2; ++side)
+			{
+				begin[side] = max(index_at(p.offsets, p.offsets_wide, 2 * pair + side), (int64_t)0);
+				end[side] = min(index_at(p.offsets, p.offsets_wide, 2 * pair + side + 1), p.rows);
+				double t = 0.0;
+				long long n = 0;
+				for (int64_t r = begin[side] + threadIdx.x; r < end[side]; r += kPairThreads)
+					if (p.saved[p.rows + r] != 0.0F)
+					{
+						t += (double)p.logp[r];
+						++n;
+					}
+				#pragma unroll
+				for (int o = 16; o > 0; o >>= 1)
+				{
+					t += __shfl_xor_sync(0xffffffffu, t, o);
+					n += __shfl_xor_sync(0xffffffffu, n, o);
+				}
+				if ((threadIdx.x & 31) == 0)
+				{
+					s_sum[side][threadIdx.x >> 5] = t;
+					s_count[side][threadIdx.x >> 5] = n;
+				}
+			}
+			__syncthreads();
+			float share[2], ratio[2];
+			double gap[2];
+			#pragma unroll
+			for (int side = 0; side < 2; ++side)
+			{
+				sum[side] = 0.0;
+				count[side] = 0;
+				for (int i = 0; i < kPairThreads / 32; ++i)
+				{
+					sum[side] += s_sum[side][i];
+					count[side] += s_count[side][i];
+				}
+				const double by = p.average && count[side] > 0 ? 1.0 / (double)count[side] : 1.0;
+				share[side] = (float)by;
+				gap[side] = sum[side] * by - (double)__ldg(p.ref_logp + 2 * pair + side);
+				ratio[side] = (float)gap[side];
+			}
+			const double h = gap[0] - gap[1];
+			float loss, dh;
+			if (p.kind == NNF_PREFERENCE_SQUARED)
+			{
+				const float off = (float)(h - 0.5 / (double)p.beta);
+				loss = off * off;
+				dh = 2.0F * off;
+			}
+			else
+			{
+				const float m = (float)(h * (double)p.beta);
+				loss = (1.0F - p.smoothing) * softplus(-m) + p.smoothing * softplus(m);
+				dh = p.beta * (p.smoothing / (1.0F + expf(-m)) - (1.0F - p.smoothing) / (1.0F + expf(m)));
+			}
+			if (threadIdx.x == 0)
+			{
+				p.loss[pair] = loss * p.scale;
+				p.rewards[2 * pair] = p.beta * ratio[0];
+				p.rewards[2 * pair + 1] = p.beta * ratio[1];
+			}
+			#pragma unroll
+			for (int side = 0; side < 2; ++side)
+			{
+				const float g = (side == 0 ? -dh : dh) * p.scale * share[side];
+				for (int64_t r = begin[side] + threadIdx.x; r < end[side]; r += kPairThreads)
+					p.dlogp[r] = p.saved[p.rows + r] != 0.0F ? g : 0.0F;
+			}
+		}
+
+		// ---- launches -------------------------------------------------------------------------------------
+		int element_size(int type)
+		{
+			switch (type)
+			{
+			case NNF_F32: case NNF_I32: return 4;
+			case NNF_BF16: case NNF_F16: return 2;
+			case NNF_I64: return 8;
+			default: return 0;
+			}
+		}
+
+		bool is_index(int type) { return type == NNF_I32 || type == NNF_I64; }
+		bool is_float(int type) { return type == NNF_F32 || type == NNF_BF16 || type == NNF_F16; }
+		bool misaligned(const void * p, int size) { return reinterpret_cast<uintptr_t>(p) % size != 0; }
+
+		// 0: fine
+		int check_rows(const char * who, const char * what, const nnf_matrix * m, bool (*of)(int))
+		{
+			if (!m)
+				return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: %s: null pointer", who, what);
+			if (!of(m->type))
+				return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: %s: type %d", who, what, (int)m->type);
+			if (m->rows < 0 || m->cols <= 0 || (m->rows > 1 && m->stride < m->cols))
+				return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: %s: bad extents rows=%lld cols=%lld stride=%lld", who, what, (long long)m->rows, (long long)m->cols, (long long)m->stride);
+			if (m->rows > 0 && !m->data)
+				return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: %s: null pointer", who, what);
+			if (misaligned(m->data, element_size(m->type)))
+				return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: %s: misaligned buffer", who, what);
+			return NNF_OK;
+		}
+
+		int check_indices(const char * who, const char * what, const nnf_indices * t)
+		{
+			if (!t || !t->data)
+				return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: %s: null pointer", who, what);
+			if (!is_index(t->type))
+				return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: %s: type %d", who, what, (int)t->type);
+			if (misaligned(t->data, element_size(t->type)))
+				return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: %s: misaligned buffer", who, what);
+			return NNF_OK;
+		}
+
+		// logits, and their gradient if there is one
+		int check_logits(const char * who, const nnf_matrix * x, const nnf_matrix * dx, int add, float temperature)
+		{
+			int st = check_rows(who, "logits", x, is_float);
+			if (st == NNF_OK && dx)
+				st = check_rows(who, "dlogits", dx, is_float);
+			if (st != NNF_OK)
+				return st;
+			if (!(temperature > 0.0F) || !(temperature < INFINITY))
+				return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: temperature %g", who, (double)temperature);
+			// a row's frame may hold a piece more than its elements fill
+			const int64_t n = 16 / element_size(x->type);
+			if ((x->cols + 2 * n - 2) / n > int64_t(kVocabCluster) * kVocabThreads * kVocabPieces)
+				return set_error(NNF_ERR_UNSUPPORTED, "%s: rows of %lld scores: at most 1 MiB a row", who, (long long)x->cols);
+			if (dx)
+			{
+				if (dx->type != x->type || dx->rows != x->rows || dx->cols != x->cols)
+					return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: dlogits have another type or shape than the logits", who);
+				if (dx->data == x->data && x->rows > 0 && (add || dx->stride != x->stride))
+					return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: dlogits in the logits' place: with their stride, and not added to", who);
+			}
+			return NNF_OK;
+		}
+
+		template <class... P>
+		int launch_rows(void (*kernel)(P...), int64_t grid, int threads, size_t smem, int cluster, cudaStream_t s, const P&... args)
+		{
+			cudaLaunchAttribute attr[2];
+			attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+			attr[0].val.programmaticStreamSerializationAllowed = 1;
+			attr[1].id = cudaLaunchAttributeClusterDimension;
+			attr[1].val.clusterDim.x = (unsigned)cluster;
+			attr[1].val.clusterDim.y = 1;
+			attr[1].val.clusterDim.z = 1;
+			cudaLaunchConfig_t cfg = {};
+			cfg.gridDim = dim3((unsigned)grid);
+			cfg.blockDim = dim3((unsigned)threads);
+			cfg.dynamicSmemBytes = smem;
+			cfg.stream = s;
+			cfg.attrs = attr;
+			cfg.numAttrs = cluster > 1 ? 2 : 1;
+			cudaLaunchKernelEx(&cfg, kernel, args...);   // the error, if any, is picked up by check_launch
+			return check_launch("vocab_rows_kernel");
+		}
+
+		template <class T, int OP>
+		int run_rows_of(cudaStream_t s, vocab_params& p)
+		{
+			constexpr int64_t n = piece<T>::N;
+			const int64_t pieces = (p.cols + 2 * n - 2) / n;
+			int64_t cluster = 1;
+			while (cluster < kVocabCluster && pieces > cluster * 512 * kVocabPieces)
+				cluster *= 2;
+			while (cluster < kVocabCluster && p.rows * cluster < sm_count() && pieces > cluster * 512)
+				cluster *= 2;
+			const int64_t per = div_up(pieces, cluster);
+			const int np = per <= 32 ? 1 : per <= 64 ? 2 : per <= 128 ? 4 : 8;
+			const int threads = (int)(div_up(div_up(per, np), 32) * 32);
+			p.cluster = (int)cluster;
+			size_t smem = 0;
+			if (OP == kDistill)
+				smem = size_t(p.kept) * 20 + size_t(div_up(np * threads * n, 32)) * 4;
+			const int64_t most = (int64_t(1) << 30) / cluster;
+			const int64_t grid = (p.rows < most ? p.rows : most) * cluster;
+			switch (np)
+			{
+			case 1: return launch_rows(vocab_rows_kernel<T, OP, 1>, grid, threads, smem, (int)cluster, s, p);
+			case 2: return launch_rows(vocab_rows_kernel<T, OP, 2>, grid, threads, smem, (int)cluster, s, p);
+			case 4: return launch_rows(vocab_rows_kernel<T, OP, 4>, grid, threads, smem, (int)cluster, s, p);
+			default: return launch_rows(vocab_rows_kernel<T, OP, 8>, grid, threads, smem, (int)cluster, s, p);
+			}
+		}
+
+		template <int OP>
+		int run_rows(cudaStream_t s, vocab_params& p, const nnf_matrix& x, const nnf_matrix * dx, float temperature)
+		{
+			p.x = x.data; p.ldx = x.stride;
+			p.dx = dx ? dx->data : nullptr; p.lddx = dx ? dx->stride : 0;
+			p.rows = x.rows; p.cols = (int)x.cols;
+			p.tau = temperature;
+			p.inv_tau = 1.0F / temperature;
+			p.k = 1.44269502162933349609375F / temperature;
+			switch (x.type)
+			{
+			case NNF_F32: return run_rows_of<float, OP>(s, p);
+			case NNF_BF16: return run_rows_of<__nv_bfloat16, OP>(s, p);
+			default: return run_rows_of<__half, OP>(s, p);
+			}
+		}
+
+		int run_bwd(cudaStream_t s, vocab_bwd_params& p, const nnf_matrix& dx, const nnf_matrix& x, float temperature)
+		{
+			p.x = x.data; p.ldx = x.stride;
+			p.dx = dx.data; p.lddx = dx.stride;
+			p.rows = x.rows; p.cols = (int)x.cols;
+			p.inv_tau = 1.0F / temperature;
+			p.k = 1.44269502162933349609375F / temperature;
+			const int64_t n = 16 / element_size(x.type), pieces = (x.cols + 2 * n - 2) / n;
+			const int threads = pieces < kBwdThreads * kBwdPieces ? (int)div_up(div_up(pieces, kBwdPieces), 32) * 32 : kBwdThreads;
+			p.slices = (int)div_up(pieces, threads * kBwdPieces);
+			const int64_t grid = x.rows * p.slices;
+			if (grid > 0x7fffffff)
+				return set_error(NNF_ERR_UNSUPPORTED, "token log probabilities, backward: too many rows");
+			switch (x.type)
+			{
+			case NNF_F32: launch(vocab_bwd_kernel<float>, grid, threads, 0, s, p); break;
+			case NNF_BF16: launch(vocab_bwd_kernel<__nv_bfloat16>, grid, threads, 0, s, p); break;
+			default: launch(vocab_bwd_kernel<__half>, grid, threads, 0, s, p); break;
+			}
+			return check_launch("vocab_bwd_kernel");
+		}
+	}
+}
+
+using namespace nnf;
+
+extern "C" int nnf_token_logp_fwd(nnf_stream_t stream, float * logp, float * saved, const nnf_matrix * logits, const nnf_indices * tokens, float temperature)
+{
+	const char * const who = "nnf_token_logp_fwd";
+	int st = check_logits(who, logits, nullptr, 0, temperature);
+	if (st != NNF_OK || logits->rows == 0)
+		return st;
+	if ((st = check_indices(who, "tokens", tokens)) != NNF_OK)
+		return st;
+	if (!logp)
+		return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+	vocab_params p = {};
+	p.logp = logp; p.saved = saved;
+	p.tokens = tokens->data; p.tokens_wide = tokens->type == NNF_I64;
+	return run_rows<kScore>((cudaStream_t)stream, p, *logits, nullptr, temperature);
+}
+
+extern "C" int nnf_token_logp_bwd(nnf_stream_t stream, const nnf_matrix * dlogits, const float * dlogp, const nnf_matrix * logits, const nnf_indices * tokens,
+	const float * saved, float temperature, int add_to_destination)
+{
+	const char * const who = "nnf_token_logp_bwd";
+	if (!dlogits)
+		return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: dlogits: null pointer", who);
+	int st = check_logits(who, logits, dlogits, add_to_destination, temperature);
+	if (st != NNF_OK || logits->rows == 0)
+		return st;
+	if ((st = check_indices(who, "tokens", tokens)) != NNF_OK)
+		return st;
+	if (!dlogp || !saved)
+		return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+	vocab_bwd_params p = {};
+	p.tokens = tokens->data; p.tokens_wide = tokens->type == NNF_I64;
+	p.dlogp = dlogp; p.saved = saved;
+	p.add = add_to_destination ? 1 : 0;
+	return run_bwd((cudaStream_t)stream, p, *dlogits, *logits, temperature);
+}
+
+extern "C" int nnf_policy_loss(nnf_stream_t stream, float * loss, float * logp, float * kl, const nnf_matrix * dlogits, const nnf_matrix * logits,
+	const nnf_indices * tokens, const float * old_logp, const float * advantages, const float * ref_logp, const float * mask,
+	float clip_low, float clip_high, float kl_coef, float temperature, float scale, int add_to_destination)
+{
+	const char * const who = "nnf_policy_loss";
+	int st = check_logits(who, logits, dlogits, add_to_destination, temperature);
+	if (st != NNF_OK)
+		return st;
+	if (!(clip_low >= 0.0F) || !(clip_low <= 1.0F) || !(clip_high >= 0.0F))
+		return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: ratios are held in [1 - %g, 1 + %g]", who, (double)clip_low, (double)clip_high);
+	if (logits->rows == 0)
+		return NNF_OK;
+	if ((st = check_indices(who, "tokens", tokens)) != NNF_OK)
+		return st;
+	if (!loss || !logp || !old_logp || !advantages)
+		return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+	vocab_params p = {};
+	p.loss = loss; p.logp = logp; p.kl = kl;
+	p.tokens = tokens->data; p.tokens_wide = tokens->type == NNF_I64;
+	p.old_logp = old_logp; p.advantages = advantages; p.ref_logp = ref_logp; p.mask = mask;
+	p.low = 1.0F - clip_low; p.high = 1.0F + clip_high; p.kl_coef = kl_coef;
+	p.scale = scale;
+	p.add = add_to_destination ? 1 : 0;
+	return run_rows<kPolicy>((cudaStream_t)stream, p, *logits, dlogits, temperature);
+}
+
+extern "C" int nnf_preference_loss(nnf_stream_t stream, float * loss, float * rewards, float * logp, float * saved, float * dlogp, const nnf_matrix * dlogits,
+	const nnf_matrix * logits, const nnf_indices * tokens, const nnf_indices * offsets, int64_t pairs, const float * ref_logp, int kind, float beta,
+	float label_smoothing, int average, float temperature, float scale, int add_to_destination)
+{
+	const char * const who = "nnf_preference_loss";
+	int st = check_logits(who, logits, dlogits, add_to_destination, temperature);
+	if (st != NNF_OK)
+		return st;
+	if (kind != NNF_PREFERENCE_LOGISTIC && kind != NNF_PREFERENCE_SQUARED)
+		return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: kind %d", who, kind);
+	if (!(beta > 0.0F) || !(beta < INFINITY) || !(label_smoothing >= 0.0F) || !(label_smoothing <= 1.0F) || pairs < 0)
+		return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: beta %g, label smoothing %g, %lld pairs", who, (double)beta, (double)label_smoothing, (long long)pairs);
+	if (pairs == 0)
+		return NNF_OK;
+	if (pairs > 0x3fffffff)
+		return set_error(NNF_ERR_UNSUPPORTED, "%s: %lld pairs", who, (long long)pairs);
+	if ((st = check_indices(who, "offsets", offsets)) != NNF_OK)
+		return st;
+	if (logits->rows > 0 && (st = check_indices(who, "tokens", tokens)) != NNF_OK)
+		return st;
+	if (!loss || !rewards || !ref_logp || (logits->rows > 0 && (!logp || !saved || !dlogp)))
+		return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+	const cudaStream_t s = (cudaStream_t)stream;
+	if (logits->rows > 0)
+	{
+		vocab_params p = {};
+		p.logp = logp; p.saved = saved;
+		p.tokens = tokens->data; p.tokens_wide = tokens->type == NNF_I64;
+		p.offsets = offsets->data; p.offsets_wide = offsets->type == NNF_I64; p.sequences = 2 * pairs;
+		if ((st = run_rows<kScore>(s, p, *logits, nullptr, temperature)) != NNF_OK)
+			return st;
+	}
+	pair_params q = {};
+	q.logp = logp; q.saved = saved; q.ref_logp = ref_logp;
+	q.offsets = offsets->data; q.offsets_wide = offsets->type == NNF_I64;
+	q.rows = logits->rows;
+	q.loss = loss; q.rewards = rewards; q.dlogp = dlogp;
+	q.beta = beta; q.smoothing = label_smoothing; q.scale = scale;
+	q.kind = kind; q.average = average ? 1 : 0;
+	launch(vocab_pair_kernel, pairs, kPairThreads, 0, s, q);
+	if ((st = check_launch("vocab_pair_kernel")) != NNF_OK || !dlogits || logits->rows == 0)
+		return st;
+	vocab_bwd_params b = {};
+	b.tokens = tokens->data; b.tokens_wide = tokens->type == NNF_I64;
+	b.dlogp = dlogp; b.saved = saved;
+	b.add = add_to_destination ? 1 : 0;
+	b.offsets = offsets->data; b.offsets_wide = offsets->type == NNF_I64; b.sequences = 2 * pairs;
+	return run_bwd(s, b, *dlogits, *logits, temperature);
+}
+
+extern "C" int nnf_distill_topk_loss(nnf_stream_t stream, float * loss, const nnf_matrix * dlogits, const nnf_matrix * logits, const nnf_matrix * teacher_ids,
+	const nnf_matrix * teacher_logits, const float * mask, float temperature, float scale, int add_to_destination)
+{
+	const char * const who = "nnf_distill_topk_loss";
+	int st = check_logits(who, logits, dlogits, add_to_destination, temperature);
+	if (st == NNF_OK)
+		st = check_rows(who, "teacher ids", teacher_ids, is_index);
+	if (st == NNF_OK)
+		st = check_rows(who, "teacher logits", teacher_logits, is_float);
+	if (st != NNF_OK)
+		return st;
+	if (teacher_ids->rows != logits->rows || teacher_logits->rows != logits->rows || teacher_ids->cols != teacher_logits->cols)
+		return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: the teacher's ids and logits are [rows][kept]", who);
+	if (teacher_ids->cols > kMaxKept)
+		return set_error(NNF_ERR_UNSUPPORTED, "%s: %lld logits kept: at most %d", who, (long long)teacher_ids->cols, kMaxKept);
+	if (logits->rows == 0)
+		return NNF_OK;
+	if (!loss)
+		return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+	vocab_params p = {};
+	p.loss = loss; p.mask = mask;
+	p.scale = scale;
+	p.add = add_to_destination ? 1 : 0;
+	p.ids = teacher_ids->data; p.ids_wide = teacher_ids->type == NNF_I64; p.ld_ids = teacher_ids->stride;
+	p.teacher = teacher_logits->data; p.teacher_type = teacher_logits->type; p.ld_teacher = teacher_logits->stride;
+	p.kept = (int)teacher_ids->cols;
+	return run_rows<kDistill>((cudaStream_t)stream, p, *logits, dlogits, temperature);
+}

@@ -253,6 +253,75 @@ namespace
 				sequence(o, [&](PyObject * item) { out.push_back(address_of<CHECKED>(item)); });
 		}
 
+		// A tensor of the losses on a vocabulary's scores, which come in several types and are read by index: what the kernels will
+		// take it for is checked here. (null, the exception set, where it is something else)
+		const at::Tensor * tensor(PyObject * o, const char * name)
+		{
+			if (!good)
+				return nullptr;
+			if (!THPVariable_Check(o))
+			{
+				fail(PyExc_TypeError, name, "a tensor is expected");
+				return nullptr;
+			}
+			const at::Tensor& t = THPVariable_Unpack(o);
+			if (!t.is_cuda() || t.layout() != at::kStrided)
+				fail(PyExc_AssertionError, name, "a CUDA tensor is expected");
+			else if (t.device().index() != c10::cuda::current_device())
+				fail(PyExc_ValueError, name, "a tensor of the current device is expected");
+			return good ? &t : nullptr;
+		}
+
+		// fp32, contiguous, of `count` elements (None: null)
+		float * floats(PyObject * o, const char * name, int64_t count)
+		{
+			const at::Tensor * t = o == Py_None ? nullptr : tensor(o, name);
+			if (!t)
+				return nullptr;
+			if (t->scalar_type() != at::kFloat)
+				fail(PyExc_TypeError, name, "float32 is expected");
+			else if (!t->is_contiguous())
+				fail(PyExc_AssertionError, name, "tensors must be contiguous CUDA tensors");
+			else if (t->numel() != count)
+				fail(PyExc_ValueError, name, "another number of elements is expected");
+			return good ? static_cast<float *>(t->data_ptr()) : nullptr;
+		}
+
+		// rows of contiguous elements (None: null)
+		const nnf_matrix * matrix(PyObject * o, const char * name, nnf_matrix& m, bool indices = false)
+		{
+			const at::Tensor * t = o == Py_None ? nullptr : tensor(o, name);
+			if (!t)
+				return nullptr;
+			m.type = type_of(*t, name, indices);
+			if (t->dim() != 2)
+				fail(PyExc_ValueError, name, "a tensor [rows][columns] is expected");
+			else if (t->size(0) > 0 && t->size(1) > 1 && t->stride(1) != 1)
+				fail(PyExc_AssertionError, name, "the elements of a row must be contiguous");
+			if (!good)
+				return nullptr;
+			m.data = t->data_ptr();
+			m.rows = t->size(0);
+			m.cols = t->size(1);
+			m.stride = m.rows > 1 ? t->stride(0) : m.cols;
+			return &m;
+		}
+
+		// a contiguous list of indices
+		const nnf_indices * indices(PyObject * o, const char * name, nnf_indices& i, int64_t count)
+		{
+			const at::Tensor * t = tensor(o, name);
+			if (!t)
+				return nullptr;
+			i.type = type_of(*t, name, true);
+			if (!t->is_contiguous())
+				fail(PyExc_AssertionError, name, "tensors must be contiguous CUDA tensors");
+			else if (t->numel() != count)
+				fail(PyExc_ValueError, name, "another number of elements is expected");
+			i.data = good ? t->data_ptr() : nullptr;
+			return &i;
+		}
+
 		template <class F>
 		void sequence(PyObject * o, F f)
 		{
@@ -266,6 +335,13 @@ namespace
 				f(PySequence_Fast_GET_ITEM(s.object, k));
 		}
 
+		void fail(PyObject * type, const char * name, const char * text)
+		{
+			if (good)
+				PyErr_Format(type, "%s: %s", name, text);
+			good = false;
+		}
+
 		void fail(PyObject * type, const char * text)
 		{
 			if (good && type)   // null: the exception is set already
@@ -274,6 +350,21 @@ namespace
 		}
 
 	private:
+		int type_of(const at::Tensor& t, const char * name, bool indices)
+		{
+			switch (t.scalar_type())
+			{
+			case at::kFloat: if (!indices) return NNF_F32; break;
+			case at::kBFloat16: if (!indices) return NNF_BF16; break;
+			case at::kHalf: if (!indices) return NNF_F16; break;
+			case at::kInt: if (indices) return NNF_I32; break;
+			case at::kLong: if (indices) return NNF_I64; break;
+			default: break;
+			}
+			fail(PyExc_TypeError, name, indices ? "int32 or int64 is expected" : "float32, bfloat16 or float16 is expected");
+			return -1;
+		}
+
 		void * address_in(PyObject * number)
 		{
 			void * p = PyLong_AsVoidPtr(number);
@@ -778,6 +869,89 @@ namespace
 		return call(a, [&] { return nnf_softmax_nll_fwd(s, probs, err, logits, targets, mask, scale, e.n, e.c, e.hw); });
 	}
 
+	NNF_NATIVE(token_logp_fwd)   // logp, saved, logits, tokens, temperature, stream
+	{
+		NNF_READ;
+		nnf_matrix x = {};
+		nnf_indices t = {};
+		PyObject * const o_logp = a.next(), * const o_saved = a.next();
+		const nnf_matrix * logits = a.matrix(a.next(), "logits", x);
+		const nnf_indices * tokens = a.indices(a.next(), "tokens", t, x.rows);
+		float * logp = a.floats(o_logp, "logp", x.rows), * saved = a.floats(o_saved, "saved", 2 * x.rows);
+		const float tau = (float)a.number();
+		const nnf_stream_t s = a.stream();
+		return call(a, [&] { return nnf_token_logp_fwd(s, logp, saved, logits, tokens, tau); });
+	}
+
+	NNF_NATIVE(token_logp_bwd)   // dlogits, dlogp, logits, tokens, saved, temperature, add_to_destination, stream
+	{
+		NNF_READ;
+		nnf_matrix x = {}, dx = {};
+		nnf_indices t = {};
+		const nnf_matrix * dlogits = a.matrix(a.next(), "dlogits", dx);
+		PyObject * const o_dlogp = a.next();
+		const nnf_matrix * logits = a.matrix(a.next(), "logits", x);
+		const nnf_indices * tokens = a.indices(a.next(), "tokens", t, x.rows);
+		const float * saved = a.floats(a.next(), "saved", 2 * x.rows), * dlogp = a.floats(o_dlogp, "dlogp", x.rows);
+		const float tau = (float)a.number();
+		const int add = a.flag();
+		const nnf_stream_t s = a.stream();
+		return call(a, [&] { return nnf_token_logp_bwd(s, dlogits, dlogp, logits, tokens, saved, tau, add); });
+	}
+
+	NNF_NATIVE(policy_loss)   // loss, logp, kl, dlogits, logits, tokens, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coef, temperature, scale, add, stream
+	{
+		NNF_READ;
+		nnf_matrix x = {}, dx = {};
+		nnf_indices t = {};
+		PyObject * const o_loss = a.next(), * const o_logp = a.next(), * const o_kl = a.next();
+		const nnf_matrix * dlogits = a.matrix(a.next(), "dlogits", dx), * logits = a.matrix(a.next(), "logits", x);
+		const nnf_indices * tokens = a.indices(a.next(), "tokens", t, x.rows);
+		float * loss = a.floats(o_loss, "loss", x.rows), * logp = a.floats(o_logp, "logp", x.rows), * kl = a.floats(o_kl, "kl", x.rows);
+		const float * old_logp = a.floats(a.next(), "old_logp", x.rows), * advantages = a.floats(a.next(), "advantages", x.rows);
+		const float * ref_logp = a.floats(a.next(), "ref_logp", x.rows), * mask = a.floats(a.next(), "mask", x.rows);
+		const float low = (float)a.number(), high = (float)a.number(), kl_coef = (float)a.number(), tau = (float)a.number(), scale = (float)a.number();
+		const int add = a.flag();
+		const nnf_stream_t s = a.stream();
+		return call(a, [&] { return nnf_policy_loss(s, loss, logp, kl, dlogits, logits, tokens, old_logp, advantages, ref_logp, mask, low, high, kl_coef, tau, scale, add); });
+	}
+
+	NNF_NATIVE(preference_loss)   // loss, rewards, logp, saved, dlogp, dlogits, logits, tokens, offsets, ref_logp, kind, beta, label_smoothing, average, temperature, scale, add, stream
+	{
+		NNF_READ;
+		nnf_matrix x = {}, dx = {};
+		nnf_indices t = {}, f = {};
+		PyObject * const o_loss = a.next(), * const o_rewards = a.next(), * const o_logp = a.next(), * const o_saved = a.next(), * const o_dlogp = a.next();
+		const int64_t pairs = a.numel(o_loss);
+		const nnf_matrix * dlogits = a.matrix(a.next(), "dlogits", dx), * logits = a.matrix(a.next(), "logits", x);
+		const nnf_indices * tokens = a.indices(a.next(), "tokens", t, x.rows), * offsets = a.indices(a.next(), "offsets", f, 2 * pairs + 1);
+		float * loss = a.floats(o_loss, "loss", pairs), * rewards = a.floats(o_rewards, "rewards", 2 * pairs), * logp = a.floats(o_logp, "logp", x.rows);
+		float * saved = a.floats(o_saved, "saved", 2 * x.rows), * dlogp = a.floats(o_dlogp, "dlogp", x.rows);
+		const float * ref_logp = a.floats(a.next(), "ref_logp", 2 * pairs);
+		const int kind = (int)a.integer();
+		const float beta = (float)a.number(), smoothing = (float)a.number();
+		const int average = a.flag();
+		const float tau = (float)a.number(), scale = (float)a.number();
+		const int add = a.flag();
+		const nnf_stream_t s = a.stream();
+		return call(a, [&] { return nnf_preference_loss(s, loss, rewards, logp, saved, dlogp, dlogits, logits, tokens, offsets, pairs, ref_logp, kind, beta, smoothing, average, tau, scale, add); });
+	}
+
+	NNF_NATIVE(distill_topk_loss)   // loss, dlogits, logits, teacher_ids, teacher_logits, mask, temperature, scale, add, stream
+	{
+		NNF_READ;
+		nnf_matrix x = {}, dx = {}, ids = {}, top = {};
+		PyObject * const o_loss = a.next();
+		const nnf_matrix * dlogits = a.matrix(a.next(), "dlogits", dx), * logits = a.matrix(a.next(), "logits", x);
+		const nnf_matrix * teacher_ids = a.matrix(a.next(), "teacher_ids", ids, true), * teacher_logits = a.matrix(a.next(), "teacher_logits", top);
+		float * loss = a.floats(o_loss, "loss", x.rows);
+		const float * mask = a.floats(a.next(), "mask", x.rows);
+		const float tau = (float)a.number(), scale = (float)a.number();
+		const int add = a.flag();
+		const nnf_stream_t s = a.stream();
+		return call(a, [&] { return nnf_distill_topk_loss(s, loss, dlogits, logits, teacher_ids, teacher_logits, mask, tau, scale, add); });
+	}
+
 	// The fields of one chunk's dict. A step hands over hundreds of chunks, so the dict is walked once and its keys, which are interned
 	// strings in nearly every program, are told apart by address; other strings are compared. (Seven look-ups per chunk took
 	// 110 ns, three times the GPU's time for a network of small layers; the walk takes 60.) Any other mapping, a subclass of dict among
@@ -978,6 +1152,7 @@ namespace
 		NNF_ENTRY_AS("nll_fwd", loss_fwd<nnf_nll_fwd>), NNF_ENTRY_AS("nll_bwd", loss_bwd<nnf_nll_bwd>),
 		NNF_ENTRY_AS("cross_entropy_fwd", loss_fwd<nnf_cross_entropy_fwd>), NNF_ENTRY_AS("cross_entropy_bwd", loss_bwd<nnf_cross_entropy_bwd>),
 		NNF_ENTRY(softmax_nll_fwd), NNF_ENTRY_AS("softmax_nll_bwd", loss_bwd<nnf_softmax_nll_bwd>), NNF_ENTRY(apply_gradient),
+		NNF_ENTRY(token_logp_fwd), NNF_ENTRY(token_logp_bwd), NNF_ENTRY(policy_loss), NNF_ENTRY(preference_loss), NNF_ENTRY(distill_topk_loss),
 		NNF_ENTRY(tester_forward), NNF_ENTRY(updater_forward), NNF_ENTRY(object_forward), NNF_ENTRY(object_backward_data),
 		NNF_ENTRY(object_backward_weights), NNF_ENTRY(object_backward_data_and_weights),
 		{"set_types", set_types, METH_VARARGS, nullptr},
