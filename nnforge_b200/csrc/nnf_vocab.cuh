@@ -27,6 +27,14 @@ namespace nnf
 		static __device__ __forceinline__ float value(const float * p) { return *p; }
 		static __device__ __forceinline__ void store(float * p, float v) { *p = v; }
 		static constexpr uint32_t kNothing = 0xff800000u;   // -infinity, in every element of the word
+		template <int K> static __device__ __forceinline__ float maximum(const uint4 (&v)[K])
+		{
+			float m = -INFINITY;
+			#pragma unroll
+			for (int j = 0; j < K; ++j)
+				m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(v[j].x), __uint_as_float(v[j].y)), fmaxf(__uint_as_float(v[j].z), __uint_as_float(v[j].w))));
+			return m;
+		}
 	};
 
 	template <> struct piece<__nv_bfloat16>
@@ -57,6 +65,16 @@ namespace nnf
 		static __device__ __forceinline__ float value(const __nv_bfloat16 * p) { return __bfloat162float(*p); }
 		static __device__ __forceinline__ void store(__nv_bfloat16 * p, float v) { *p = __float2bfloat16_rn(v); }
 		static constexpr uint32_t kNothing = 0xff80ff80u;
+		// two elements at a time; NaN is passed over, as fmaxf does
+		template <int K> static __device__ __forceinline__ float maximum(const uint4 (&v)[K])
+		{
+			auto two = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162 *>(&w); };
+			__nv_bfloat162 m = __hmax2(__hmax2(two(v[0].x), two(v[0].y)), __hmax2(two(v[0].z), two(v[0].w)));
+			#pragma unroll
+			for (int j = 1; j < K; ++j)
+				m = __hmax2(m, __hmax2(__hmax2(two(v[j].x), two(v[j].y)), __hmax2(two(v[j].z), two(v[j].w))));
+			return fmaxf(__bfloat162float(m.x), __bfloat162float(m.y));
+		}
 	};
 
 	template <> struct piece<__half>
@@ -88,6 +106,16 @@ namespace nnf
 		static __device__ __forceinline__ float value(const __half * p) { return __half2float(*p); }
 		static __device__ __forceinline__ void store(__half * p, float v) { *p = __float2half_rn(v); }
 		static constexpr uint32_t kNothing = 0xfc00fc00u;
+		// two elements at a time; NaN is passed over, as fmaxf does
+		template <int K> static __device__ __forceinline__ float maximum(const uint4 (&v)[K])
+		{
+			auto two = [](uint32_t w) { return *reinterpret_cast<const __half2 *>(&w); };
+			__half2 m = __hmax2(__hmax2(two(v[0].x), two(v[0].y)), __hmax2(two(v[0].z), two(v[0].w)));
+			#pragma unroll
+			for (int j = 1; j < K; ++j)
+				m = __hmax2(m, __hmax2(__hmax2(two(v[j].x), two(v[j].y)), __hmax2(two(v[j].z), two(v[j].w))));
+			return fmaxf(__half2float(m.x), __half2float(m.y));
+		}
 	};
 
 	// The 16-byte frame of a row of `cols` elements that starts anywhere: every aligned piece that holds one of its elements. Only the
@@ -157,13 +185,81 @@ namespace nnf
 		return part_m == m ? 1.0F : exp2_of((part_m - m) * k);
 	}
 
-	__device__ __forceinline__ softmax_part join(const softmax_part& a, const softmax_part& b, float k)
+	// sum of exp2((x - m)*k) over some pieces whose maximum is at most m; m = -infinity: of 0 (or NaN)
+	template <class T, int K>
+	__device__ __forceinline__ float sum_of_exp(const uint4 (&v)[K], float m, float k)
 	{
-		softmax_part r;
-		r.m = fmaxf(a.m, b.m);
-		r.s = a.s * rescale(a.m, r.m, k) + b.s * rescale(b.m, r.m, k);
-		return r;
+		constexpr int N = piece<T>::N;
+		const float base = m == -INFINITY ? 0.0F : m;
+		const float mk = base * k;
+		float s[2] = {0.0F, 0.0F};
+		if (fabsf(mk) < 1.0e6F)
+		{
+			// One fused operation for the argument, x*k - mk, where mk is m*k rounded: the sum is against 2^mk, and what mk is off by
+			// (2^-24 of it: 1e-6 for scores of 10, 0.04 at the limit) is put right on the sum.
+			#pragma unroll
+			for (int j = 0; j < K; ++j)
+			{
+				float f[N];
+				piece<T>::unpack(v[j], f);
+				#pragma unroll
+				for (int e = 0; e < N; ++e)
+					s[e & 1] += exp2_of(__fmaf_rn(f[e], k, -mk));
+			}
+			return (s[0] + s[1]) * exp2_of(-__fmaf_rn(base, k, -mk));
+		}
+		// larger ones (a row of nothing but the type's lowest value): the difference first
+		#pragma unroll
+		for (int j = 0; j < K; ++j)
+		{
+			float f[N];
+			piece<T>::unpack(v[j], f);
+			#pragma unroll
+			for (int e = 0; e < N; ++e)
+				s[e & 1] += exp2_of((f[e] - base) * k);
+		}
+		return s[0] + s[1];
 	}
+
+	// The gradient's c*exp2((x - m)*k) over a row. As in sum_of_exp the argument is one fused operation, and what m*k rounded is off by goes
+	// into c; fp32 results take the product with c, 16-bit ones have it in the argument (log2 |c| - m*k, rounded, is off by 2^-24 of
+	// at most 400: 1.7e-5 of the result, against the 2^-9 or 2^-12 of their own rounding) and their sign in the packed words.
+	template <class T>
+	struct row_gradient
+	{
+		float m, k, c, mk, offset;
+		uint32_t sign;
+
+		__device__ __forceinline__ row_gradient(float m, float k, float c) : m(m), k(k), c(c), mk(m * k)
+		{
+			const float put_right = c * exp2_of(-__fmaf_rn(m, k, -mk));
+			offset = sizeof(T) == 4 ? put_right : __log2f(fabsf(put_right)) - mk;
+			sign = c < 0.0F ? 0x80008000u : 0u;
+		}
+		__device__ __forceinline__ bool near() const { return fabsf(mk) < (sizeof(T) == 4 ? 1.0e6F : 256.0F); }
+
+		__device__ __forceinline__ uint4 whole(const uint4& v) const   // near() only
+		{
+			constexpr int N = piece<T>::N;
+			float f[N];
+			piece<T>::unpack(v, f);
+			#pragma unroll
+			for (int e = 0; e < N; ++e)
+				f[e] = sizeof(T) == 4 ? exp2_of(__fmaf_rn(f[e], k, -mk)) * offset : exp2_of(__fmaf_rn(f[e], k, offset));
+			uint4 w = piece<T>::pack(f);
+			if (sizeof(T) == 2)
+				w = make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);
+			return w;
+		}
+
+		__device__ __forceinline__ void values(const uint4& v, float (&f)[piece<T>::N]) const
+		{
+			piece<T>::unpack(v, f);
+			#pragma unroll
+			for (int e = 0; e < piece<T>::N; ++e)
+				f[e] = exp2_of((f[e] - m) * k) * c;
+		}
+	};
 
 	__device__ __forceinline__ float vocab_warp_max(float v)
 	{

@@ -114,6 +114,38 @@ namespace nnf
 			}
 		}
 
+		// what a policy's row comes to
+		struct policy_row
+		{
+			float logp, kl, loss;
+			float c, at_token;   // the gradient: c*exp2((x_j - M)*k), and at the token
+		};
+
+		__device__ __forceinline__ policy_row policy_of(const vocab_params& p, float xa, const softmax_part& total, float weight, float old_logp, float a, float ref_logp, bool on)
+		{
+			policy_row r = {0.0F, 0.0F, 0.0F, 0.0F, 0.0F};
+			if (!on)
+				return r;
+			r.logp = (xa - total.m) * p.inv_tau - logf(total.s);
+			const float ratio = expf(r.logp - old_logp);
+			const float free = ratio * a, held = fminf(fmaxf(ratio, p.low), p.high) * a;
+			// min() that keeps a NaN
+			float loss = -(free <= held ? free : held < free ? held : free + held);
+			float g = held < free ? 0.0F : free;
+			if (p.ref_logp)
+			{
+				const float gap = ref_logp - r.logp, grown = expm1f(gap);
+				r.kl = grown - gap;
+				loss += p.kl_coef * r.kl;
+				g += p.kl_coef * grown;
+			}
+			g = weight != 0.0F ? g * weight * p.inv_tau : 0.0F;
+			r.loss = weight != 0.0F ? loss * weight : 0.0F;
+			r.c = -g / total.s;
+			r.at_token = -g * expm1f(r.logp);   // g * (1 - p)
+			return r;
+		}
+
 		struct distill_shared
 		{
 			int * id;         // -1: the entry does not count
@@ -295,33 +327,15 @@ namespace nnf
 				const float weight = p.scale * w;
 				if (OP == kPolicy)
 				{
-					float logp = 0.0F, kl = 0.0F, loss = 0.0F;
-					if (on)
-					{
-						logp = (xa - total.m) * p.inv_tau - logf(total.s);
-						const float a = __ldg(p.advantages + row), ratio = expf(logp - __ldg(p.old_logp + row));
-						const float free = ratio * a, held = fminf(fmaxf(ratio, p.low), p.high) * a;
-						// min() that keeps a NaN
-						loss = -(free <= held ? free : held < free ? held : free + held);
-						float g = held < free ? 0.0F : free;
-						if (p.ref_logp)
-						{
-							const float gap = __ldg(p.ref_logp + row) - logp, grown = expm1f(gap);
-							kl = grown - gap;
-							loss += p.kl_coef * kl;
-							g += p.kl_coef * grown;
-						}
-						g = weight != 0.0F ? g * weight * p.inv_tau : 0.0F;
-						loss = weight != 0.0F ? loss * weight : 0.0F;
-						c = -g / total.s;
-						at_token = -g * expm1f(logp);   // g * (1 - p)
-					}
+					const policy_row l = policy_of(p, xa, total, weight, __ldg(p.old_logp + row), __ldg(p.advantages + row), p.ref_logp ? __ldg(p.ref_logp + row) : 0.0F, on);
+					c = l.c;
+					at_token = l.at_token;
 					if (first)
 					{
-						p.loss[row] = loss;
-						p.logp[row] = logp;
+						p.loss[row] = l.loss;
+						p.logp[row] = l.logp;
 						if (p.kl)
-							p.kl[row] = kl;
+							p.kl[row] = l.kl;
 					}
 					on = on && at_token != 0.0F | c != 0.0F;
 				}
@@ -425,6 +439,393 @@ namespace nnf
 						}
 					}
 					__syncthreads();
+				}
+			}
+		}
+
+		constexpr unsigned long long kWaitNs = 5000000000ull;
+
+		__device__ __forceinline__ uint32_t shared_address(const void * p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+		__device__ __forceinline__ void mbar_init(uint64_t * b, int count)
+		{
+			asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(shared_address(b)), "r"(count) : "memory");
+		}
+		__device__ __forceinline__ void mbar_arrive(uint64_t * b)
+		{
+			asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(shared_address(b)) : "memory");
+		}
+		__device__ __forceinline__ void mbar_arrive_expect(uint64_t * b, uint32_t bytes)
+		{
+			asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(shared_address(b)), "r"(bytes) : "memory");
+		}
+		__device__ __forceinline__ bool mbar_try(uint64_t * b, uint32_t phase)
+		{
+			uint32_t done;
+			asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+				: "=r"(done) : "r"(shared_address(b)), "r"(phase) : "memory");
+			return done != 0;
+		}
+		// Bounded: when the limit runs out the error word is raised and the caller carries on, without waiting any more; every loop has
+		// its number of turns from the start, so that all threads still meet at the same barriers and leave.
+		__device__ __forceinline__ void mbar_wait(uint64_t * b, uint32_t phase, bool& gave_up, int * error)
+		{
+			if (gave_up || mbar_try(b, phase))
+				return;
+			unsigned long long start, now;
+			asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
+			while (!mbar_try(b, phase))
+			{
+				asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+				if (now - start > kWaitNs)
+				{
+					gave_up = true;
+					if (error)
+						*error = 4;
+					return;
+				}
+			}
+		}
+
+		__device__ __forceinline__ void copy_bulk(void * to, const void * from, uint32_t bytes, uint64_t * bar)
+		{
+			asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+				:: "r"(shared_address(to)), "l"(from), "r"(bytes), "r"(shared_address(bar)) : "memory");
+		}
+
+		// ---- long rows: held in shared memory ----------------------------------------------------------------------------
+		// A CTA per row (a cluster, where the row is split), several of them on an SM. Bulk copies bring the row in, chunk by chunk; each
+		// chunk's exponentials are summed against the thread's running maximum as it arrives; the gradient is computed from shared memory.
+		// What an SM has in flight are the rows of its other CTAs.
+		constexpr int kHeldThreads = 256, kHeldChunk = 4, kHeldChunks = 32;   // pieces of a chunk that a thread takes
+
+		struct held_params
+		{
+			vocab_params v;
+			int slice_pieces;
+			int * error;
+		};
+
+		struct held_result     // what the row comes to, found by the first warp
+		{
+			float m, c, at_token, share;
+			int on;
+		};
+
+		template <class T, int OP>
+		__global__ void __launch_bounds__(kHeldThreads, 3) vocab_held_kernel(const held_params hp)
+		{
+			constexpr int N = piece<T>::N;
+			extern __shared__ __align__(128) unsigned char s_held[];
+			__shared__ softmax_part s_part[kVocabCluster * (kHeldThreads / 32)];
+			__shared__ uint64_t s_bar[kHeldChunks];
+			__shared__ held_result s_result;
+			__shared__ float s_red[2][kHeldThreads / 32];
+			const vocab_params& p = hp.v;
+			const uint32_t split = (uint32_t)p.cluster;
+			const uint32_t rank = split > 1 ? vocab_cluster_rank() : 0;
+			const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+			const int64_t row = blockIdx.x / split;
+			if (split > 1)
+				vocab_cluster_arrive();   // waited for before the first store into another CTA
+			const row_frame<T> x(const_cast<T *>(static_cast<const T *>(p.x)) + row * p.ldx, p.cols);
+			T * const dx = p.dx ? static_cast<T *>(p.dx) + row * p.lddx : nullptr;
+			const bool aligned = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x.at)) & 15) == 0;
+			const int per = split > 1 ? (x.pieces + (int)split - 1) / (int)split : x.pieces;
+			const int from = (int)rank * per, count = min(per, x.pieces - from);   // this CTA's pieces (none: count <= 0)
+			const int chunk = (int)blockDim.x * kHeldChunk, chunks = (count + chunk - 1) / chunk;
+			uint4 * const held = reinterpret_cast<uint4 *>(s_held);
+			if (threadIdx.x == 0)
+			{
+				for (int i = 0; i < chunks; ++i)
+					mbar_init(s_bar + i, 1);
+				asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+			}
+			pdl_begin();
+
+			const float w = p.mask ? __ldg(p.mask + row) : 1.0F;
+			int token = 0;
+			bool on = w != 0.0F;
+			if (OP == kPolicy)
+			{
+				const int64_t t = index_at(p.tokens, p.tokens_wide, row);
+				on = on && t >= 0 && t < p.cols;
+				token = on ? (int)t : 0;
+			}
+			const float weight = p.scale * w;
+			if (!on)   // the same in every CTA of the cluster
+			{
+				if (rank == 0 && threadIdx.x == 0)
+				{
+					p.loss[row] = 0.0F;
+					if (OP == kPolicy)
+					{
+						p.logp[row] = 0.0F;
+						if (p.kl)
+							p.kl[row] = 0.0F;
+					}
+				}
+				if (dx && !p.add)
+					for (int i = threadIdx.x; i < count; i += blockDim.x)
+						store_piece<T>(x, dx, aligned, from + i, 0, [](int) { return 0.0F; });
+				if (split > 1)
+					vocab_cluster_wait();
+				return;
+			}
+			if (threadIdx.x == 0)
+			{
+				for (int i = 0; i < chunks; ++i)
+				{
+					int a = i * chunk, b = min(a + chunk, count);
+					a += a == 0 && !x.whole(from);
+					b -= b == count && b > a && !x.whole(from + b - 1);
+					const uint32_t bytes = b > a ? (uint32_t)(b - a) * 16 : 0;
+					mbar_arrive_expect(s_bar + i, bytes);
+					if (bytes)
+						copy_bulk(held + a, x.address(from + a), bytes, s_bar + i);
+				}
+			}
+			// a partial piece is fetched by the thread that works on it
+			if (count > 0 && threadIdx.x == 0 && !x.whole(from))
+				held[0] = x.load(from);
+			if (count > 1 && (int)threadIdx.x == (count - 1) % (int)blockDim.x && !x.whole(from + count - 1))
+				held[count - 1] = x.load(from + count - 1);
+			const float xa = OP == kPolicy && warp == 0 ? piece<T>::value(x.at + token) : 0.0F;
+			distill_shared d = {};
+			float t_max = 0.0F, t_sum = 0.0F;
+			if (OP == kDistill)
+			{
+				d.id = reinterpret_cast<int *>(held + hp.slice_pieces);
+				d.q = reinterpret_cast<float *>(d.id + p.kept);
+				d.old = d.q + p.kept;
+				d.x = d.old + p.kept;
+				d.seen = reinterpret_cast<uint32_t *>(d.x + p.kept);
+				for (int i = threadIdx.x; i < (hp.slice_pieces * N + 31) / 32; i += blockDim.x)
+					d.seen[i] = 0;
+				// the teacher's row, while the student's is on its way
+				float m = -INFINITY;
+				for (int e = threadIdx.x; e < p.kept; e += blockDim.x)
+				{
+					const int64_t id = index_at(p.ids, p.ids_wide, row * p.ld_ids + e);
+					const bool in = id >= 0 && id < p.cols;
+					const float t = in ? value_at(p.teacher, p.teacher_type, row * p.ld_teacher + e) : -INFINITY;
+					const int at = in ? ((int)id + x.shift) / N - from : -1;
+					d.id[e] = in ? (int)id : -1;
+					d.q[e] = t;
+					if (in && rank == 0 && at >= count)
+						d.x[e] = piece<T>::value(x.at + id);   // another CTA's column: the loss is found here
+					if (p.add && at >= 0 && at < count)
+						d.old[e] = piece<T>::value(dx + id);
+					m = fmaxf(m, t);
+				}
+				m = vocab_warp_max(m);
+				if (lane == 0)
+					s_red[0][warp] = m;
+				__syncthreads();
+				for (int i = 0; i < warps; ++i)
+					m = fmaxf(m, s_red[0][i]);
+				t_max = m == -INFINITY ? 0.0F : m;
+				float s = 0.0F;
+				for (int e = threadIdx.x; e < p.kept; e += blockDim.x)
+					s += exp2_of((d.q[e] - t_max) * p.k);
+				s = vocab_warp_sum(s);
+				if (lane == 0)
+					s_red[1][warp] = s;
+				__syncthreads();
+				for (int i = 0; i < warps; ++i)
+					t_sum += s_red[1][i];
+			}
+			else
+				__syncthreads();   // the barriers are there
+
+			// ---- maximum and sum, against the thread's running maximum ----
+			softmax_part part = {-INFINITY, 0.0F};
+			bool gave_up = false;
+			for (int i = 0; i < chunks; ++i)
+			{
+				mbar_wait(s_bar + i, 0, gave_up, hp.error);
+				uint4 v[kHeldChunk];
+				#pragma unroll
+				for (int j = 0; j < kHeldChunk; ++j)
+				{
+					const int at = i * chunk + j * (int)blockDim.x + (int)threadIdx.x;
+					v[j] = at < count ? held[at] : make_uint4(piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing);
+				}
+				const float m = fmaxf(part.m, piece<T>::template maximum<kHeldChunk>(v));
+				part.s *= rescale(part.m, m, p.k);
+				part.m = m;
+				part.s += sum_of_exp<T, kHeldChunk>(v, m, p.k);
+			}
+			if (gave_up)
+			{
+				bool again = false;   // nobody leaves while a copy may still write into this CTA's shared memory
+				for (int i = 0; i < chunks; ++i)
+					mbar_wait(s_bar + i, 0, again, hp.error);
+			}
+			{
+				const float m = vocab_warp_max(part.m);
+				part.s = vocab_warp_sum(part.s * rescale(part.m, m, p.k));
+				part.m = m;
+			}
+			// the first warp of every CTA gets every warp's part
+			if (split > 1)
+			{
+				vocab_cluster_wait();
+				if (lane < (int)split)
+					vocab_cluster_store(s_part + rank * warps + warp, lane, part);
+				vocab_cluster_arrive();
+				vocab_cluster_wait();
+			}
+			else
+			{
+				if (lane == 0)
+					s_part[warp] = part;
+				__syncthreads();
+			}
+			if (warp == 0)
+			{
+				softmax_part total = {-INFINITY, 0.0F};
+				for (int i = lane; i < (int)split * warps; i += 32)
+					total.m = fmaxf(total.m, s_part[i].m);
+				total.m = vocab_warp_max(total.m);
+				for (int i = lane; i < (int)split * warps; i += 32)
+					total.s += s_part[i].s * rescale(s_part[i].m, total.m, p.k);
+				total.s = vocab_warp_sum(total.s);
+				on = total.s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
+				held_result r = {total.m, 0.0F, 0.0F, 0.0F, on};
+				if (OP == kPolicy)
+				{
+					const policy_row l = policy_of(p, xa, total, weight, __ldg(p.old_logp + row), __ldg(p.advantages + row), p.ref_logp ? __ldg(p.ref_logp + row) : 0.0F, on);
+					r.c = l.c;
+					r.at_token = l.at_token;
+					r.on = l.c != 0.0F || l.at_token != 0.0F;
+					if (rank == 0 && lane == 0)
+					{
+						p.loss[row] = l.loss;
+						p.logp[row] = l.logp;
+						if (p.kl)
+							p.kl[row] = l.kl;
+					}
+				}
+				else
+				{
+					on = on && t_sum != 0.0F && weight != 0.0F;
+					r.on = on;
+					r.c = on ? -weight * p.tau / total.s : 0.0F;
+					r.share = on ? weight * p.tau / t_sum : 0.0F;
+					if (rank == 0)
+					{
+						float sum = 0.0F;
+						if (on)
+						{
+							const float ln = logf(total.s), t_ln = logf(t_sum);
+							for (int e = lane; e < p.kept; e += 32)
+							{
+								const float z = (d.q[e] - t_max) * p.inv_tau;
+								const float q = exp2_of((d.q[e] - t_max) * p.k);
+								if (q != 0.0F)
+								{
+									const int at = d.id[e] + x.shift - from * N;
+									const float xe = at < count * N ? piece<T>::value(reinterpret_cast<const T *>(held) + at) : d.x[e];
+									sum += q * ((z - t_ln) - ((xe - total.m) * p.inv_tau - ln));
+								}
+							}
+							sum = vocab_warp_sum(sum) * (weight * p.tau * p.tau / t_sum);
+						}
+						if (lane == 0)
+							p.loss[row] = sum;
+					}
+				}
+				if (lane == 0)
+					s_result = r;
+			}
+			__syncthreads();
+			const held_result r = s_result;
+			if (!dx)
+				return;
+			if (!r.on)
+			{
+				if (!p.add)
+					for (int i = threadIdx.x; i < count; i += blockDim.x)
+						store_piece<T>(x, dx, aligned, from + i, 0, [](int) { return 0.0F; });
+				return;
+			}
+			const int token_piece = OP == kPolicy ? (token + x.shift) / N - from : -1, token_place = (token + x.shift) % N;
+			const row_gradient<T> gradient(r.m, p.k, r.c);
+			if (aligned && !p.add && gradient.near())
+			{
+				// whole pieces; then the partial ones, and the token over what its piece's thread has just written
+				const int lo = count > 0 && !x.whole(from) ? 1 : 0, hi = count > 0 && !x.whole(from + count - 1) ? count - 1 : count;
+				uint4 * const to = reinterpret_cast<uint4 *>(dx - x.shift) + from;
+				#pragma unroll 4
+				for (int i = threadIdx.x; i < hi; i += blockDim.x)
+					if (i >= lo)
+						__stcs(to + i, gradient.whole(held[i]));
+				auto edge = [&](int i)
+				{
+					float f[N];
+					gradient.values(held[i], f);
+					store_piece<T>(x, dx, true, from + i, 0, [&](int e) { return f[e]; });
+				};
+				if (lo > 0 && threadIdx.x == 0)
+					edge(0);
+				if (hi < count && hi >= lo && (int)threadIdx.x == hi % (int)blockDim.x)
+					edge(hi);
+				if (OP == kPolicy && token_piece >= 0 && token_piece < count && (int)threadIdx.x == token_piece % (int)blockDim.x)
+					piece<T>::store(dx + token, r.at_token);
+			}
+			else
+				for (int i = threadIdx.x; i < count; i += blockDim.x)
+				{
+					float f[N];
+					gradient.values(held[i], f);
+					if (OP == kPolicy && i == token_piece)
+					{
+						#pragma unroll
+						for (int e = 0; e < N; ++e)
+							f[e] = e == token_place ? r.at_token : f[e];
+					}
+					store_piece<T>(x, dx, aligned, from + i, p.add, [&](int e) { return f[e]; });
+				}
+			if (OP == kDistill)
+			{
+				// The columns that the teacher kept: c*(q - p), written over -c*p. An index that is there twice holds the sum of both; the
+				// first of its entries writes it. `seen` shows whether there is one at all.
+				bool twice = false;
+				for (int e = threadIdx.x; e < p.kept; e += blockDim.x)
+				{
+					const int at = d.id[e] < 0 ? -1 : d.id[e] + x.shift - from * N;
+					if (at >= 0 && at < count * N)
+					{
+						const uint32_t bit = 1u << (at & 31);
+						twice = twice || (atomicOr(d.seen + (at >> 5), bit) & bit);
+					}
+				}
+				twice = __syncthreads_or(twice);   // also: the pieces above are written
+				for (int e = threadIdx.x; e < p.kept; e += blockDim.x)
+				{
+					const int id = d.id[e], at = id < 0 ? -1 : id + x.shift - from * N;
+					if (at >= 0 && at < count * N)
+					{
+						float q = exp2_of((d.q[e] - t_max) * p.k);
+						bool leads = true;
+						if (twice)
+						{
+							q = 0.0F;
+							for (int o = 0; o < p.kept; ++o)
+								if (d.id[o] == id)
+								{
+									leads = leads && o >= e;
+									q += exp2_of((d.q[o] - t_max) * p.k);
+								}
+						}
+						if (leads)
+						{
+							const float xe = piece<T>::value(reinterpret_cast<const T *>(held) + at);
+							const float g = exp2_of((xe - r.m) * p.k) * r.c + r.share * q;
+							piece<T>::store(dx + id, p.add ? d.old[e] + g : g);
+						}
+					}
 				}
 			}
 		}
@@ -704,8 +1105,42 @@ namespace nnf
 		}
 
 		template <class T, int OP>
+		int run_held(cudaStream_t s, const vocab_params& v, int64_t pieces)
+		{
+			int64_t cluster = 1;
+			while (cluster < kVocabCluster && pieces > cluster * 4200)
+				cluster *= 2;
+			if (tune().vocab_split > 0)
+				cluster = tune().vocab_split;
+			held_params p = {};
+			p.v = v;
+			p.v.cluster = (int)cluster;
+			const int64_t per = div_up(pieces, cluster);
+			p.slice_pieces = (int)((per + 7) & ~int64_t(7));
+			p.error = device_error_word();
+			int threads = (int)(div_up(div_up(per, 16), 32) * 32);
+			threads = threads < 64 ? 64 : threads > kHeldThreads ? kHeldThreads : threads;
+			const size_t smem = size_t(p.slice_pieces) * 16 + (OP == kDistill ? size_t(v.kept) * 16 + size_t(div_up(int64_t(p.slice_pieces) * piece<T>::N, 32)) * 4 : 0);
+			auto kernel = vocab_held_kernel<T, OP>;
+			const int limit = running_config().max_shared_memory_per_block_optin - 4096;
+			if (smem > (size_t)limit)
+				return set_error(NNF_ERR_UNSUPPORTED, "vocab_held_kernel: %lld bytes", (long long)smem);
+			// the attribute is the kernel's: the same value whatever the shape, so that host threads do not lower it under each other's launches
+			const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
+			if (e != cudaSuccess)
+				return set_error(NNF_ERR_CUDA, "vocab_held_kernel: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+			return launch_rows(kernel, v.rows * cluster, threads, smem, (int)cluster, s, p);
+		}
+
+		template <class T, int OP>
 		int run_rows_of(cudaStream_t s, vocab_params& p)
 		{
+			if constexpr (OP != kScore)
+			{
+				const int64_t pieces = (p.cols + 2 * int64_t(piece<T>::N) - 2) / piece<T>::N;
+				if (tune().vocab_form == 2 || (tune().vocab_form != 1 && pieces > 256))
+					return run_held<T, OP>(s, p, pieces);
+			}
 			constexpr int64_t n = piece<T>::N;
 			const int64_t pieces = (p.cols + 2 * n - 2) / n;
 			int64_t cluster = 1;

@@ -22,6 +22,16 @@ def capi():
     return capi
 
 
+@pytest.fixture(autouse=True, params=["built-in choice", "registers", "shared memory", "shared memory, split"])
+def form(request, capi):
+    """Every test runs in each form of the kernels, whatever the sizes for which it is chosen."""
+    capi.set_tuning("vocab_form", {"b": 0, "r": 1, "s": 2}[request.param[0]])
+    capi.set_tuning("vocab_split", 4 if "split" in request.param else 0)
+    yield
+    assert capi.fused_error_check() == 0
+    capi.set_tuning("reset", 0)
+
+
 def generator(salt):
     g = torch.Generator(device="cuda")
     g.manual_seed(1234 + salt)
