@@ -178,6 +178,30 @@ namespace nnf
 		return e;
 	}
 
+	// two fp32 operations in one instruction, each rounded as by itself
+	__device__ __forceinline__ unsigned long long pair_of(float a, float b)
+	{
+		unsigned long long r;
+		asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+		return r;
+	}
+	__device__ __forceinline__ void pair_apart(unsigned long long p, float& a, float& b)
+	{
+		asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+	}
+	__device__ __forceinline__ unsigned long long pair_fma(unsigned long long a, unsigned long long b, unsigned long long c)
+	{
+		unsigned long long r;
+		asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+		return r;
+	}
+	__device__ __forceinline__ unsigned long long pair_add(unsigned long long a, unsigned long long b)
+	{
+		unsigned long long r;
+		asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+		return r;
+	}
+
 	// What a part's exponentials are multiplied with when the maximum becomes m. A part without a maximum (-infinity) keeps its sum: 0, or
 	// NaN where an element was NaN, which no maximum shows.
 	__device__ __forceinline__ float rescale(float part_m, float m, float k)
@@ -197,15 +221,22 @@ namespace nnf
 		{
 			// One fused operation for the argument, x*k - mk, where mk is m*k rounded: the sum is against 2^mk, and what mk is off by
 			// (2^-24 of it: 1e-6 for scores of 10, 0.04 at the limit) is put right on the sum.
+			const unsigned long long kk = pair_of(k, k), mm = pair_of(-mk, -mk);
+			unsigned long long both = pair_of(0.0F, 0.0F);
 			#pragma unroll
 			for (int j = 0; j < K; ++j)
 			{
 				float f[N];
 				piece<T>::unpack(v[j], f);
 				#pragma unroll
-				for (int e = 0; e < N; ++e)
-					s[e & 1] += exp2_of(__fmaf_rn(f[e], k, -mk));
+				for (int e = 0; e < N; e += 2)
+				{
+					float a, b;
+					pair_apart(pair_fma(pair_of(f[e], f[e + 1]), kk, mm), a, b);
+					both = pair_add(both, pair_of(exp2_of(a), exp2_of(b)));
+				}
 			}
+			pair_apart(both, s[0], s[1]);
 			return (s[0] + s[1]) * exp2_of(-__fmaf_rn(base, k, -mk));
 		}
 		// larger ones (a row of nothing but the type's lowest value): the difference first
@@ -243,9 +274,15 @@ namespace nnf
 			constexpr int N = piece<T>::N;
 			float f[N];
 			piece<T>::unpack(v, f);
+			const unsigned long long kk = pair_of(k, k), add = sizeof(T) == 4 ? pair_of(-mk, -mk) : pair_of(offset, offset);
 			#pragma unroll
-			for (int e = 0; e < N; ++e)
-				f[e] = sizeof(T) == 4 ? exp2_of(__fmaf_rn(f[e], k, -mk)) * offset : exp2_of(__fmaf_rn(f[e], k, offset));
+			for (int e = 0; e < N; e += 2)
+			{
+				float a, b;
+				pair_apart(pair_fma(pair_of(f[e], f[e + 1]), kk, add), a, b);
+				f[e] = sizeof(T) == 4 ? exp2_of(a) * offset : exp2_of(a);
+				f[e + 1] = sizeof(T) == 4 ? exp2_of(b) * offset : exp2_of(b);
+			}
 			uint4 w = piece<T>::pack(f);
 			if (sizeof(T) == 2)
 				w = make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);

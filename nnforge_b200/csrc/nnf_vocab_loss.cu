@@ -462,8 +462,8 @@ namespace nnf
 		__device__ __forceinline__ bool mbar_try(uint64_t * b, uint32_t phase)
 		{
 			uint32_t done;
-			asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-				: "=r"(done) : "r"(shared_address(b)), "r"(phase) : "memory");
+			asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+				: "=r"(done) : "r"(shared_address(b)), "r"(phase), "r"(1000000u) : "memory");   // suspended for up to a millisecond
 			return done != 0;
 		}
 		// Bounded: when the limit runs out the error word is raised and the caller carries on, without waiting any more; every loop has
