@@ -269,7 +269,7 @@ namespace nnf
 		}
 		__device__ __forceinline__ bool near() const { return fabsf(mk) < (sizeof(T) == 4 ? 1.0e6F : 256.0F); }
 
-		__device__ __forceinline__ uint4 whole(const uint4& v) const   // near() only
+		template <bool NEAR> __device__ __forceinline__ uint4 whole(const uint4& v) const
 		{
 			constexpr int N = piece<T>::N;
 			float f[N];
@@ -278,25 +278,34 @@ namespace nnf
 			#pragma unroll
 			for (int e = 0; e < N; e += 2)
 			{
-				float a, b;
-				pair_apart(pair_fma(pair_of(f[e], f[e + 1]), kk, add), a, b);
-				f[e] = sizeof(T) == 4 ? exp2_of(a) * offset : exp2_of(a);
-				f[e + 1] = sizeof(T) == 4 ? exp2_of(b) * offset : exp2_of(b);
+				if (NEAR)
+				{
+					float a, b;
+					pair_apart(pair_fma(pair_of(f[e], f[e + 1]), kk, add), a, b);
+					f[e] = sizeof(T) == 4 ? exp2_of(a) * offset : exp2_of(a);
+					f[e + 1] = sizeof(T) == 4 ? exp2_of(b) * offset : exp2_of(b);
+				}
+				else
+				{
+					f[e] = exp2_of((f[e] - m) * k) * c;
+					f[e + 1] = exp2_of((f[e + 1] - m) * k) * c;
+				}
 			}
 			uint4 w = piece<T>::pack(f);
-			if (sizeof(T) == 2)
+			if (NEAR && sizeof(T) == 2)
 				w = make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);
 			return w;
 		}
-
-		__device__ __forceinline__ void values(const uint4& v, float (&f)[piece<T>::N]) const
-		{
-			piece<T>::unpack(v, f);
-			#pragma unroll
-			for (int e = 0; e < piece<T>::N; ++e)
-				f[e] = exp2_of((f[e] - m) * k) * c;
-		}
 	};
+
+	// the elements of some pieces join a part
+	template <class T, int K>
+	__device__ __forceinline__ void add_part(softmax_part& part, const uint4 (&v)[K], float k)
+	{
+		const float m = fmaxf(part.m, piece<T>::template maximum<K>(v));
+		part.s = part.s * rescale(part.m, m, k) + sum_of_exp<T, K>(v, m, k);
+		part.m = m;
+	}
 
 	__device__ __forceinline__ float vocab_warp_max(float v)
 	{

@@ -13,6 +13,8 @@
 // distributed shared memory. Maximum, sum and everything behind them are fp32; a gradient is rounded once, when it is stored.
 #include "nnf_vocab.cuh"
 
+#include <type_traits>
+
 namespace nnf
 {
 	namespace
@@ -496,24 +498,29 @@ namespace nnf
 		// ---- long rows: held in shared memory ----------------------------------------------------------------------------
 		// A CTA per row (a cluster, where the row is split), several of them on an SM. Bulk copies bring the row in, chunk by chunk; each
 		// chunk's exponentials are summed against the thread's running maximum as it arrives; the gradient is computed from shared memory.
-		// What an SM has in flight are the rows of its other CTAs.
-		constexpr int kHeldThreads = 256, kHeldChunk = 4, kHeldChunks = 32;   // pieces of a chunk that a thread takes
+		// What an SM has in flight are the rows of its other CTAs: the bytes that a row takes up decide how many those are, so a
+		// quarter of a long row is held in registers.
+		constexpr int kHeldThreads = 256, kHeldChunk = 4, kHeldChunks = 40;   // kHeldChunk: pieces of a chunk that a thread takes
+
+		// kAnyRow: gradients that are added, or whose rows start elsewhere in their 16 bytes than the logits'; the loss alone.
+		// kAlignedRow: whole pieces are stored at once. kRegisterRow: and the second chunk is held in registers.
+		enum { kAnyRow = 0, kAlignedRow = 1, kRegisterRow = 2 };
 
 		struct held_params
 		{
 			vocab_params v;
-			int slice_pieces;
+			int slots;                 // pieces of a CTA in shared memory
 			int * error;
 		};
 
-		struct held_result     // what the row comes to, found by the first warp
+		struct held_result             // what the row comes to, found by the first warp
 		{
 			float m, c, at_token, share;
 			int on;
 		};
 
-		template <class T, int OP>
-		__global__ void __launch_bounds__(kHeldThreads, 3) vocab_held_kernel(const held_params hp)
+		template <class T, int OP, int ROW>
+		__global__ void __launch_bounds__(kHeldThreads, 4) vocab_held_kernel(const held_params hp)
 		{
 			constexpr int N = piece<T>::N;
 			extern __shared__ __align__(128) unsigned char s_held[];
@@ -524,18 +531,21 @@ namespace nnf
 			const vocab_params& p = hp.v;
 			const uint32_t split = (uint32_t)p.cluster;
 			const uint32_t rank = split > 1 ? vocab_cluster_rank() : 0;
-			const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+			const int tid = (int)threadIdx.x, step = (int)blockDim.x, lane = tid & 31, warp = tid >> 5, warps = step >> 5;
 			const int64_t row = blockIdx.x / split;
 			if (split > 1)
 				vocab_cluster_arrive();   // waited for before the first store into another CTA
 			const row_frame<T> x(const_cast<T *>(static_cast<const T *>(p.x)) + row * p.ldx, p.cols);
 			T * const dx = p.dx ? static_cast<T *>(p.dx) + row * p.lddx : nullptr;
-			const bool aligned = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x.at)) & 15) == 0;
 			const int per = split > 1 ? (x.pieces + (int)split - 1) / (int)split : x.pieces;
-			const int from = (int)rank * per, count = min(per, x.pieces - from);   // this CTA's pieces (none: count <= 0)
-			const int chunk = (int)blockDim.x * kHeldChunk, chunks = (count + chunk - 1) / chunk;
+			const int from = (int)rank * per, count = max(min(per, x.pieces - from), 0);   // this CTA's pieces
+			const int chunk = step * kHeldChunk;
+			const int away = ROW == kRegisterRow && count > 2 * chunk ? chunk : 0;         // of those, in registers: [chunk, 2*chunk)
+			const int kept = count - away, chunks = (kept + chunk - 1) / chunk;            // in shared memory, in their order
+			const int lo = count > 0 && !x.whole(from) ? 1 : 0, hi = count > lo && !x.whole(from + count - 1) ? count - 1 : count;   // whole pieces
 			uint4 * const held = reinterpret_cast<uint4 *>(s_held);
-			if (threadIdx.x == 0)
+			T * const held_at = reinterpret_cast<T *>(s_held);
+			if (tid == 0)
 			{
 				for (int i = 0; i < chunks; ++i)
 					mbar_init(s_bar + i, 1);
@@ -553,9 +563,30 @@ namespace nnf
 				token = on ? (int)t : 0;
 			}
 			const float weight = p.scale * w;
+			// this CTA's elements: [begin, begin + elements) of the row
+			const int begin = max(from * N - x.shift, 0), elements = max(min((from + count) * N - x.shift, p.cols) - begin, 0);
+			auto nothing = [&]()
+			{
+				if (ROW == kAnyRow)
+				{
+					if (dx && !p.add)
+						for (int e = tid; e < elements; e += step)
+							piece<T>::store(dx + begin + e, 0.0F);
+					return;
+				}
+				uint4 * const out = reinterpret_cast<uint4 *>(dx - x.shift) + from;
+				for (int i = tid + lo; i < hi; i += step)
+					__stcs(out + i, make_uint4(0, 0, 0, 0));
+				if (tid < 2 * N)
+				{
+					const int i = tid < N ? 0 : count - 1;
+					if ((tid < N ? lo > 0 : hi < count) && x.has(from + i, tid % N))
+						piece<T>::store(dx + (from + i) * N - x.shift + tid % N, 0.0F);
+				}
+			};
 			if (!on)   // the same in every CTA of the cluster
 			{
-				if (rank == 0 && threadIdx.x == 0)
+				if (rank == 0 && tid == 0)
 				{
 					p.loss[row] = 0.0F;
 					if (OP == kPolicy)
@@ -565,56 +596,70 @@ namespace nnf
 							p.kl[row] = 0.0F;
 					}
 				}
-				if (dx && !p.add)
-					for (int i = threadIdx.x; i < count; i += blockDim.x)
-						store_piece<T>(x, dx, aligned, from + i, 0, [](int) { return 0.0F; });
+				nothing();
 				if (split > 1)
 					vocab_cluster_wait();
 				return;
 			}
-			if (threadIdx.x == 0)
+			if (tid == 0)
 			{
 				for (int i = 0; i < chunks; ++i)
 				{
-					int a = i * chunk, b = min(a + chunk, count);
-					a += a == 0 && !x.whole(from);
-					b -= b == count && b > a && !x.whole(from + b - 1);
+					const int skip = i > 0 ? away : 0;
+					const int a = max(i * chunk, lo), b = min((i + 1) * chunk, hi - away);
 					const uint32_t bytes = b > a ? (uint32_t)(b - a) * 16 : 0;
 					mbar_arrive_expect(s_bar + i, bytes);
 					if (bytes)
-						copy_bulk(held + a, x.address(from + a), bytes, s_bar + i);
+						copy_bulk(held + a, x.address(from + a + skip), bytes, s_bar + i);
 				}
 			}
-			// a partial piece is fetched by the thread that works on it
-			if (count > 0 && threadIdx.x == 0 && !x.whole(from))
-				held[0] = x.load(from);
-			if (count > 1 && (int)threadIdx.x == (count - 1) % (int)blockDim.x && !x.whole(from + count - 1))
-				held[count - 1] = x.load(from + count - 1);
+			uint4 own[kHeldChunk];
+			if (ROW == kRegisterRow)
+			{
+				#pragma unroll
+				for (int j = 0; j < kHeldChunk; ++j)
+					own[j] = away ? __ldcs(x.address(from + chunk + j * step + tid))
+						: make_uint4(piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing);
+			}
+			// the partial pieces, an element a thread
+			if (tid < 2 * N)
+			{
+				const int i = tid < N ? 0 : count - 1, e = tid % N;
+				if (tid < N ? lo > 0 : hi < count)
+					held_at[(tid < N ? 0 : kept - 1) * N + e] = x.has(from + i, e) ? x.at[(from + i) * N - x.shift + e] : T(-INFINITY);
+			}
 			const float xa = OP == kPolicy && warp == 0 ? piece<T>::value(x.at + token) : 0.0F;
 			distill_shared d = {};
 			float t_max = 0.0F, t_sum = 0.0F;
+			// the score at a column of this CTA, in shared memory; elsewhere it was fetched with the teacher's row
+			auto place = [&](int id) { const int e = id + x.shift - from * N; return away && e >= 2 * chunk * N ? e - chunk * N : e; };
+			auto present = [&](int id)
+			{
+				const int e = id + x.shift - from * N;
+				return e >= 0 && e < count * N && !(away && e >= chunk * N && e < 2 * chunk * N);
+			};
 			if (OP == kDistill)
 			{
-				d.id = reinterpret_cast<int *>(held + hp.slice_pieces);
+				d.id = reinterpret_cast<int *>(held + hp.slots);
 				d.q = reinterpret_cast<float *>(d.id + p.kept);
 				d.old = d.q + p.kept;
 				d.x = d.old + p.kept;
 				d.seen = reinterpret_cast<uint32_t *>(d.x + p.kept);
-				for (int i = threadIdx.x; i < (hp.slice_pieces * N + 31) / 32; i += blockDim.x)
+				for (int i = tid; i < (count * N + 31) / 32; i += step)
 					d.seen[i] = 0;
 				// the teacher's row, while the student's is on its way
 				float m = -INFINITY;
-				for (int e = threadIdx.x; e < p.kept; e += blockDim.x)
+				for (int e = tid; e < p.kept; e += step)
 				{
 					const int64_t id = index_at(p.ids, p.ids_wide, row * p.ld_ids + e);
 					const bool in = id >= 0 && id < p.cols;
 					const float t = in ? value_at(p.teacher, p.teacher_type, row * p.ld_teacher + e) : -INFINITY;
-					const int at = in ? ((int)id + x.shift) / N - from : -1;
+					const bool mine = in && id >= begin && id < begin + elements;
 					d.id[e] = in ? (int)id : -1;
 					d.q[e] = t;
-					if (in && rank == 0 && at >= count)
-						d.x[e] = piece<T>::value(x.at + id);   // another CTA's column: the loss is found here
-					if (p.add && at >= 0 && at < count)
+					if (in && (mine || rank == 0) && !present((int)id))
+						d.x[e] = piece<T>::value(x.at + id);   // (the first CTA finds the loss)
+					if (ROW == kAnyRow && p.add && mine)
 						d.old[e] = piece<T>::value(dx + id);
 					m = fmaxf(m, t);
 				}
@@ -626,17 +671,16 @@ namespace nnf
 					m = fmaxf(m, s_red[0][i]);
 				t_max = m == -INFINITY ? 0.0F : m;
 				float s = 0.0F;
-				for (int e = threadIdx.x; e < p.kept; e += blockDim.x)
+				for (int e = tid; e < p.kept; e += step)
 					s += exp2_of((d.q[e] - t_max) * p.k);
 				s = vocab_warp_sum(s);
 				if (lane == 0)
 					s_red[1][warp] = s;
-				__syncthreads();
+			}
+			__syncthreads();   // the barriers and the partial pieces are there
+			if (OP == kDistill)
 				for (int i = 0; i < warps; ++i)
 					t_sum += s_red[1][i];
-			}
-			else
-				__syncthreads();   // the barriers are there
 
 			// ---- maximum and sum, against the thread's running maximum ----
 			softmax_part part = {-INFINITY, 0.0F};
@@ -648,14 +692,13 @@ namespace nnf
 				#pragma unroll
 				for (int j = 0; j < kHeldChunk; ++j)
 				{
-					const int at = i * chunk + j * (int)blockDim.x + (int)threadIdx.x;
-					v[j] = at < count ? held[at] : make_uint4(piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing);
+					const int at = i * chunk + j * step + tid;
+					v[j] = at < kept ? held[at] : make_uint4(piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing);
 				}
-				const float m = fmaxf(part.m, piece<T>::template maximum<kHeldChunk>(v));
-				part.s *= rescale(part.m, m, p.k);
-				part.m = m;
-				part.s += sum_of_exp<T, kHeldChunk>(v, m, p.k);
+				add_part<T, kHeldChunk>(part, v, p.k);
 			}
+			if (ROW == kRegisterRow && away)
+				add_part<T, kHeldChunk>(part, own, p.k);
 			if (gave_up)
 			{
 				bool again = false;   // nobody leaves while a copy may still write into this CTA's shared memory
@@ -721,13 +764,11 @@ namespace nnf
 							const float ln = logf(total.s), t_ln = logf(t_sum);
 							for (int e = lane; e < p.kept; e += 32)
 							{
-								const float z = (d.q[e] - t_max) * p.inv_tau;
 								const float q = exp2_of((d.q[e] - t_max) * p.k);
 								if (q != 0.0F)
 								{
-									const int at = d.id[e] + x.shift - from * N;
-									const float xe = at < count * N ? piece<T>::value(reinterpret_cast<const T *>(held) + at) : d.x[e];
-									sum += q * ((z - t_ln) - ((xe - total.m) * p.inv_tau - ln));
+									const float xe = present(d.id[e]) ? piece<T>::value(held_at + place(d.id[e])) : d.x[e];
+									sum += q * (((d.q[e] - t_max) * p.inv_tau - t_ln) - ((xe - total.m) * p.inv_tau - ln));
 								}
 							}
 							sum = vocab_warp_sum(sum) * (weight * p.tau * p.tau / t_sum);
@@ -745,86 +786,96 @@ namespace nnf
 				return;
 			if (!r.on)
 			{
-				if (!p.add)
-					for (int i = threadIdx.x; i < count; i += blockDim.x)
-						store_piece<T>(x, dx, aligned, from + i, 0, [](int) { return 0.0F; });
+				nothing();
 				return;
 			}
-			const int token_piece = OP == kPolicy ? (token + x.shift) / N - from : -1, token_place = (token + x.shift) % N;
 			const row_gradient<T> gradient(r.m, p.k, r.c);
-			if (aligned && !p.add && gradient.near())
+			if (ROW == kAnyRow)
 			{
-				// whole pieces; then the partial ones, and the token over what its piece's thread has just written
-				const int lo = count > 0 && !x.whole(from) ? 1 : 0, hi = count > 0 && !x.whole(from + count - 1) ? count - 1 : count;
-				uint4 * const to = reinterpret_cast<uint4 *>(dx - x.shift) + from;
-				#pragma unroll 4
-				for (int i = threadIdx.x; i < hi; i += blockDim.x)
-					if (i >= lo)
-						__stcs(to + i, gradient.whole(held[i]));
-				auto edge = [&](int i)
+				for (int e = tid; e < elements; e += step)
 				{
-					float f[N];
-					gradient.values(held[i], f);
-					store_piece<T>(x, dx, true, from + i, 0, [&](int e) { return f[e]; });
-				};
-				if (lo > 0 && threadIdx.x == 0)
-					edge(0);
-				if (hi < count && hi >= lo && (int)threadIdx.x == hi % (int)blockDim.x)
-					edge(hi);
-				if (OP == kPolicy && token_piece >= 0 && token_piece < count && (int)threadIdx.x == token_piece % (int)blockDim.x)
-					piece<T>::store(dx + token, r.at_token);
+					const int id = begin + e;
+					float g = exp2_of((piece<T>::value(held_at + id + x.shift - from * N) - r.m) * p.k) * r.c;
+					if (OP == kPolicy && id == token)
+						g = r.at_token;
+					piece<T>::store(dx + id, p.add ? piece<T>::value(dx + id) + g : g);
+				}
 			}
 			else
-				for (int i = threadIdx.x; i < count; i += blockDim.x)
+			{
+				uint4 * const out = reinterpret_cast<uint4 *>(dx - x.shift) + from;
+				auto pieces = [&](auto near)
 				{
-					float f[N];
-					gradient.values(held[i], f);
-					if (OP == kPolicy && i == token_piece)
+					for (int i = 0; i < chunks; ++i)
+					{
+						const int at = i * chunk + tid, skip = i > 0 ? away : 0;
+						#pragma unroll
+						for (int j = 0; j < kHeldChunk; ++j)
+							if (at + j * step >= lo && at + j * step < hi - away)
+								__stcs(out + (at + skip + j * step), gradient.template whole<near.value>(held[at + j * step]));
+					}
+					if (ROW == kRegisterRow && away)
 					{
 						#pragma unroll
-						for (int e = 0; e < N; ++e)
-							f[e] = e == token_place ? r.at_token : f[e];
+						for (int j = 0; j < kHeldChunk; ++j)
+							__stcs(out + (chunk + j * step + tid), gradient.template whole<near.value>(own[j]));
 					}
-					store_piece<T>(x, dx, aligned, from + i, p.add, [&](int e) { return f[e]; });
+				};
+				if (gradient.near())
+					pieces(std::true_type());
+				else
+					pieces(std::false_type());
+				if (tid < 2 * N)
+				{
+					const int i = tid < N ? 0 : count - 1, e = tid % N, id = (from + i) * N - x.shift + e;
+					if ((tid < N ? lo > 0 : hi < count) && x.has(from + i, e) && !(OP == kPolicy && id == token))
+						piece<T>::store(dx + id, exp2_of((piece<T>::value(held_at + (tid < N ? 0 : kept - 1) * N + e) - r.m) * p.k) * r.c);
 				}
+				if (OP == kPolicy && token >= begin && token < begin + elements)
+				{
+					// behind the token's piece, by the thread that has just written it
+					const int i = (token + x.shift) / N - from;
+					if (tid == i % step)
+						piece<T>::store(dx + token, r.at_token);
+				}
+			}
 			if (OP == kDistill)
 			{
 				// The columns that the teacher kept: c*(q - p), written over -c*p. An index that is there twice holds the sum of both; the
 				// first of its entries writes it. `seen` shows whether there is one at all.
 				bool twice = false;
-				for (int e = threadIdx.x; e < p.kept; e += blockDim.x)
+				for (int e = tid; e < p.kept; e += step)
 				{
-					const int at = d.id[e] < 0 ? -1 : d.id[e] + x.shift - from * N;
-					if (at >= 0 && at < count * N)
+					const int at = d.id[e] - begin;
+					if (d.id[e] >= 0 && at >= 0 && at < elements)
 					{
 						const uint32_t bit = 1u << (at & 31);
 						twice = twice || (atomicOr(d.seen + (at >> 5), bit) & bit);
 					}
 				}
 				twice = __syncthreads_or(twice);   // also: the pieces above are written
-				for (int e = threadIdx.x; e < p.kept; e += blockDim.x)
+				for (int e = tid; e < p.kept; e += step)
 				{
-					const int id = d.id[e], at = id < 0 ? -1 : id + x.shift - from * N;
-					if (at >= 0 && at < count * N)
+					const int id = d.id[e];
+					if (id < begin || id >= begin + elements)
+						continue;
+					float q = exp2_of((d.q[e] - t_max) * p.k);
+					bool leads = true;
+					if (twice)
 					{
-						float q = exp2_of((d.q[e] - t_max) * p.k);
-						bool leads = true;
-						if (twice)
-						{
-							q = 0.0F;
-							for (int o = 0; o < p.kept; ++o)
-								if (d.id[o] == id)
-								{
-									leads = leads && o >= e;
-									q += exp2_of((d.q[o] - t_max) * p.k);
-								}
-						}
-						if (leads)
-						{
-							const float xe = piece<T>::value(reinterpret_cast<const T *>(held) + at);
-							const float g = exp2_of((xe - r.m) * p.k) * r.c + r.share * q;
-							piece<T>::store(dx + id, p.add ? d.old[e] + g : g);
-						}
+						q = 0.0F;
+						for (int o = 0; o < p.kept; ++o)
+							if (d.id[o] == id)
+							{
+								leads = leads && o >= e;
+								q += exp2_of((d.q[o] - t_max) * p.k);
+							}
+					}
+					if (leads)
+					{
+						const float xe = present(id) ? piece<T>::value(held_at + place(id)) : d.x[e];
+						const float g = exp2_of((xe - r.m) * p.k) * r.c + r.share * q;
+						piece<T>::store(dx + id, ROW == kAnyRow && p.add ? d.old[e] + g : g);
 					}
 				}
 			}
@@ -1115,13 +1166,17 @@ namespace nnf
 			held_params p = {};
 			p.v = v;
 			p.v.cluster = (int)cluster;
-			const int64_t per = div_up(pieces, cluster);
-			p.slice_pieces = (int)((per + 7) & ~int64_t(7));
 			p.error = device_error_word();
+			const int64_t per = div_up(pieces, cluster);
 			int threads = (int)(div_up(div_up(per, 16), 32) * 32);
 			threads = threads < 64 ? 64 : threads > kHeldThreads ? kHeldThreads : threads;
-			const size_t smem = size_t(p.slice_pieces) * 16 + (OP == kDistill ? size_t(v.kept) * 16 + size_t(div_up(int64_t(p.slice_pieces) * piece<T>::N, 32)) * 4 : 0);
-			auto kernel = vocab_held_kernel<T, OP>;
+			const int64_t chunk = int64_t(threads) * kHeldChunk;
+			const bool aligned = v.dx && !v.add && ((reinterpret_cast<uintptr_t>(v.dx) ^ reinterpret_cast<uintptr_t>(v.x)) & 15) == 0 &&
+				(v.rows < 2 || (v.lddx - v.ldx) * (int64_t)sizeof(T) % 16 == 0);
+			const bool registers = aligned && threads == kHeldThreads && per >= 3 * chunk && tune().vocab_regs != 99;
+			p.slots = (int)((per - (registers ? chunk : 0) + 7) & ~int64_t(7));
+			const size_t smem = size_t(p.slots) * 16 + (OP == kDistill ? size_t(v.kept) * 16 + size_t(div_up(per * piece<T>::N, 32)) * 4 : 0);
+			auto kernel = registers ? vocab_held_kernel<T, OP, kRegisterRow> : aligned ? vocab_held_kernel<T, OP, kAlignedRow> : vocab_held_kernel<T, OP, kAnyRow>;
 			const int limit = running_config().max_shared_memory_per_block_optin - 4096;
 			if (smem > (size_t)limit)
 				return set_error(NNF_ERR_UNSUPPORTED, "vocab_held_kernel: %lld bytes", (long long)smem);
