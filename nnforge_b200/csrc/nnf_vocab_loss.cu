@@ -881,6 +881,126 @@ namespace nnf
 			}
 		}
 
+		// ---- log probabilities alone: nothing to be held -----------------------------------------------------------------
+		// A CTA per row (a cluster, where there are few rows); a thread's next pieces are on their way while it sums the current ones.
+		constexpr int kScoreThreads = 256, kScorePieces = 4;
+
+		template <class T>
+		__global__ void __launch_bounds__(kScoreThreads, 4) vocab_score_kernel(const vocab_params p)
+		{
+			constexpr int N = piece<T>::N;
+			__shared__ softmax_part s_part[kVocabCluster * (kScoreThreads / 32)];
+			const uint32_t split = (uint32_t)p.cluster;
+			const uint32_t rank = split > 1 ? vocab_cluster_rank() : 0;
+			const int tid = (int)threadIdx.x, step = (int)blockDim.x, lane = tid & 31, warp = tid >> 5, warps = step >> 5;
+			const int64_t row = blockIdx.x / split;
+			if (split > 1)
+				vocab_cluster_arrive();
+			const row_frame<T> x(const_cast<T *>(static_cast<const T *>(p.x)) + row * p.ldx, p.cols);
+			const int per = split > 1 ? (x.pieces + (int)split - 1) / (int)split : x.pieces;
+			const int from = (int)rank * per, to = min(from + per, x.pieces);
+			const int lo = from + (from < to && !x.whole(from)), hi = to - (to > lo && !x.whole(to - 1));   // whole pieces
+			pdl_begin();
+			bool inside = true;
+			if (p.offsets)
+			{
+				int64_t begin, end;
+				covered_rows(p, begin, end);
+				inside = row >= begin && row < end;
+			}
+			const int64_t token = inside ? index_at(p.tokens, p.tokens_wide, row) : -1;
+			if (token < 0 || token >= p.cols)   // the same in every CTA of the cluster
+			{
+				if (inside && rank == 0 && tid == 0)
+				{
+					p.logp[row] = 0.0F;
+					if (p.saved)
+						p.saved[row] = p.saved[p.rows + row] = 0.0F;
+				}
+				if (split > 1)
+					vocab_cluster_wait();
+				return;
+			}
+			const uint4 nothing = make_uint4(piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing);
+			const uint4 * const in = x.address(0);
+			uint4 v[kScorePieces], next[kScorePieces];
+			#pragma unroll
+			for (int j = 0; j < kScorePieces; ++j)
+			{
+				const int at = lo + j * step + tid;
+				v[j] = at < hi ? __ldg(in + at) : nothing;
+			}
+			float xa = 0.0F;
+			softmax_part part = {-INFINITY, 0.0F};
+			if (rank == 0 && tid == 0)
+				xa = piece<T>::value(x.at + token);
+			if (tid < 2 * N && from < to)
+			{
+				// the partial pieces, an element a thread
+				const int at = tid < N ? from : to - 1, e = tid % N;
+				if ((tid < N ? lo > from : hi < to) && x.has(at, e))
+				{
+					part.m = piece<T>::value(x.at + at * N - x.shift + e);
+					part.s = part.m == -INFINITY ? 0.0F : part.m - part.m + 1.0F;   // NaN stays
+					if (!(part.m == part.m))
+						part.m = -INFINITY;
+				}
+			}
+			for (int i = lo; i < hi; i += kScorePieces * step)
+			{
+				#pragma unroll
+				for (int j = 0; j < kScorePieces; ++j)
+				{
+					const int at = i + (kScorePieces + j) * step + tid;
+					next[j] = at < hi ? __ldg(in + at) : nothing;
+				}
+				add_part<T, kScorePieces>(part, v, p.k);
+				#pragma unroll
+				for (int j = 0; j < kScorePieces; ++j)
+					v[j] = next[j];
+			}
+			{
+				const float m = vocab_warp_max(part.m);
+				part.s = vocab_warp_sum(part.s * rescale(part.m, m, p.k));
+				part.m = m;
+			}
+			if (split > 1)
+			{
+				// the first CTA gets every warp's part
+				vocab_cluster_wait();
+				if (lane == 0)
+					vocab_cluster_store(s_part + rank * warps + warp, 0, part);
+				vocab_cluster_arrive();
+				vocab_cluster_wait();
+			}
+			else
+			{
+				if (lane == 0)
+					s_part[warp] = part;
+				__syncthreads();
+			}
+			if (rank == 0 && warp == 0)
+			{
+				softmax_part total = {-INFINITY, 0.0F};
+				for (int i = lane; i < (int)split * warps; i += 32)
+					total.m = fmaxf(total.m, s_part[i].m);
+				total.m = vocab_warp_max(total.m);
+				for (int i = lane; i < (int)split * warps; i += 32)
+					total.s += s_part[i].s * rescale(s_part[i].m, total.m, p.k);
+				total.s = vocab_warp_sum(total.s);
+				if (lane == 0)
+				{
+					const bool on = total.s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
+					p.logp[row] = on ? (xa - total.m) * p.inv_tau - logf(total.s) : 0.0F;
+					if (p.saved)
+					{
+						p.saved[row] = on ? total.m : 0.0F;
+						p.saved[p.rows + row] = on ? total.s : 0.0F;
+					}
+				}
+			}
+		}
+
 		// ---- backward of the log probabilities: one pass, nothing to be found first ------------------------
 		struct vocab_bwd_params
 		{
@@ -1190,7 +1310,24 @@ namespace nnf
 		template <class T, int OP>
 		int run_rows_of(cudaStream_t s, vocab_params& p)
 		{
-			if constexpr (OP != kScore)
+			if constexpr (OP == kScore)
+			{
+				if (tune().vocab_form != 1)
+				{
+					const int64_t pieces = (p.cols + 2 * int64_t(piece<T>::N) - 2) / piece<T>::N;
+					int64_t cluster = 1;
+					while (cluster < kVocabCluster && p.rows * cluster < 2 * sm_count() && pieces > cluster * 512)
+						cluster *= 2;
+					if (tune().vocab_split > 0)
+						cluster = tune().vocab_split;
+					const int64_t per = div_up(pieces, cluster);
+					int threads = (int)(div_up(div_up(per, 8), 32) * 32);
+					threads = threads < 32 ? 32 : threads > kScoreThreads ? kScoreThreads : threads;
+					p.cluster = (int)cluster;
+					return launch_rows(vocab_score_kernel<T>, p.rows * cluster, threads, 0, (int)cluster, s, p);
+				}
+			}
+			else
 			{
 				const int64_t pieces = (p.cols + 2 * int64_t(piece<T>::N) - 2) / piece<T>::N;
 				if (tune().vocab_form == 2 || (tune().vocab_form != 1 && pieces > 256))
