@@ -298,6 +298,11 @@ namespace nnf
 		}
 	};
 
+	__device__ __forceinline__ softmax_part part_of(float x)
+	{
+		return {fmaxf(x, -INFINITY), x == -INFINITY ? 0.0F : x - x + 1.0F};   // (infinity and NaN: NaN)
+	}
+
 	// the elements of some pieces join a part
 	template <class T, int K>
 	__device__ __forceinline__ void add_part(softmax_part& part, const uint4 (&v)[K], float k)
@@ -309,10 +314,9 @@ namespace nnf
 
 	__device__ __forceinline__ float vocab_warp_max(float v)
 	{
-		#pragma unroll
-		for (int o = 16; o > 0; o >>= 1)
-			v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-		return v;
+		float r;
+		asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+		return r;
 	}
 
 	__device__ __forceinline__ float vocab_warp_sum(float v)

@@ -19,10 +19,8 @@ namespace nnf
 {
 	namespace
 	{
-		constexpr int kVocabPieces = 8;          // 16-byte pieces of a row that a thread holds
-		constexpr int kVocabThreads = 1024;      // most threads of a CTA
 		constexpr int kVocabCluster = 8;         // most CTAs of a row (the portable cluster size)
-		constexpr int kVocabWarps = kVocabThreads / 32;
+		constexpr int64_t kMaxPieces = 65536;    // of a row: 1 MiB
 		constexpr int kMaxKept = 1024;           // most logits that are kept of a teacher's row
 
 		enum { kScore = 0, kPolicy = 1, kDistill = 2 };
@@ -148,6 +146,15 @@ namespace nnf
 			return r;
 		}
 
+		// of a row's partial pieces an element a lane: the first piece's in the lower half of the warp, the last one's in the upper
+		template <class T>
+		__device__ __forceinline__ float edge_of(const row_frame<T>& x, int lane)
+		{
+			const int at = lane < 16 ? 0 : x.pieces - 1, e = lane & 15;
+			const bool there = e < piece<T>::N && !x.whole(at) && (lane < 16 || x.pieces > 1) && x.has(at, e);
+			return there ? piece<T>::value(x.at + at * piece<T>::N - x.shift + e) : -INFINITY;
+		}
+
 		struct distill_shared
 		{
 			int * id;         // -1: the entry does not count
@@ -157,293 +164,6 @@ namespace nnf
 			float * old;      // what the gradient held (it is added to)
 			uint32_t * seen;  // a bit for each of this CTA's columns
 		};
-
-		// NP: pieces of a thread
-		template <class T, int OP, int NP>
-		__global__ void __launch_bounds__(kVocabThreads) vocab_rows_kernel(const vocab_params p)
-		{
-			constexpr int N = piece<T>::N;
-			extern __shared__ __align__(16) unsigned char s_dyn[];
-			__shared__ softmax_part s_part[2][kVocabCluster * kVocabWarps];
-			pdl_begin();
-
-			const uint32_t split = (uint32_t)p.cluster;
-			const uint32_t rank = split > 1 ? vocab_cluster_rank() : 0;
-			const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-			const int parts = (int)split * warps;
-			const int64_t row_step = gridDim.x / split;
-			if (split > 1)
-			{
-				vocab_cluster_arrive();   // every CTA of the cluster has started before the first store into another one
-				vocab_cluster_wait();
-			}
-			distill_shared d = {};
-			if (OP == kDistill)
-			{
-				d.id = reinterpret_cast<int *>(s_dyn);
-				d.q = reinterpret_cast<float *>(d.id + p.kept);
-				d.lnq = d.q + p.kept;
-				d.x = d.lnq + p.kept;
-				d.old = d.x + p.kept;
-				d.seen = reinterpret_cast<uint32_t *>(d.old + p.kept);
-				const int words = (NP * (int)blockDim.x * N + 31) / 32;
-				for (int i = threadIdx.x; i < words; i += blockDim.x)
-					d.seen[i] = 0;
-			}
-			int64_t begin = 0, end = p.rows;
-			if (OP == kScore && p.offsets)
-				covered_rows(p, begin, end);
-
-			int phase = 0;
-			for (int64_t row = begin + blockIdx.x / split; row < end; row += row_step)
-			{
-				const row_frame<T> x(const_cast<T *>(static_cast<const T *>(p.x)) + row * p.ldx, p.cols);
-				T * const dx = p.dx ? static_cast<T *>(p.dx) + row * p.lddx : nullptr;
-				const bool aligned = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x.at)) & 15) == 0;
-				const int per = (x.pieces + (int)split - 1) / (int)split;
-				const int from = (int)rank * per, to = min(from + per, x.pieces);   // this CTA's pieces
-
-				const float w = OP != kScore && p.mask ? __ldg(p.mask + row) : 1.0F;
-				int64_t token = 0;
-				bool on = w != 0.0F;
-				if (OP != kDistill)
-				{
-					token = index_at(p.tokens, p.tokens_wide, row);
-					on = on && token >= 0 && token < p.cols;
-				}
-				softmax_part total = {0.0F, 0.0F};
-				float xa = 0.0F;
-				uint4 v[NP];
-				bool any = false;
-				if (on)
-				{
-					#pragma unroll
-					for (int j = 0; j < NP; ++j)
-					{
-						const int i = from + j * (int)blockDim.x + (int)threadIdx.x;
-						v[j] = make_uint4(piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing);
-						if (i < to)
-							v[j] = x.load(i);
-					}
-					if (OP != kDistill)
-						xa = piece<T>::value(x.at + token);
-					else if (warp == 0)
-					{
-						// the teacher's probabilities over the logits that are kept: one warp, while the row is on its way
-						float m = -INFINITY;
-						for (int e = lane; e < p.kept; e += 32)
-						{
-							const int64_t id = index_at(p.ids, p.ids_wide, row * p.ld_ids + e);
-							const bool in = id >= 0 && id < p.cols;
-							const float t = in ? value_at(p.teacher, p.teacher_type, row * p.ld_teacher + e) : -INFINITY;
-							const int i = in ? (int)(id + x.shift) / N : -1;
-							d.id[e] = in ? (int)id : -1;
-							d.lnq[e] = t;
-							d.x[e] = in && (rank == 0 || (i >= from && i < to)) ? piece<T>::value(x.at + id) : 0.0F;
-							if (p.add && i >= from && i < to)
-								d.old[e] = piece<T>::value(dx + id);
-							m = fmaxf(m, t);
-						}
-						m = vocab_warp_max(m);
-						const float base = m == -INFINITY ? 0.0F : m;
-						float s = 0.0F;
-						for (int e = lane; e < p.kept; e += 32)
-							s += d.q[e] = expf((d.lnq[e] - base) * p.inv_tau);
-						s = vocab_warp_sum(s);
-						const float r = 1.0F / s, ln = logf(s);
-						for (int e = lane; e < p.kept; e += 32)
-						{
-							d.q[e] = s == 0.0F ? 0.0F : d.q[e] * r;
-							d.lnq[e] = (d.lnq[e] - base) * p.inv_tau - ln;
-						}
-						any = s != 0.0F;
-					}
-
-					float m = -INFINITY;
-					#pragma unroll
-					for (int j = 0; j < NP; ++j)
-					{
-						float f[N];
-						piece<T>::unpack(v[j], f);
-						#pragma unroll
-						for (int e = 0; e < N; ++e)
-							m = fmaxf(m, f[e]);
-					}
-					softmax_part part;
-					part.m = vocab_warp_max(m);
-					const float base = part.m == -INFINITY ? 0.0F : part.m;
-					part.s = 0.0F;
-					#pragma unroll
-					for (int j = 0; j < NP; ++j)
-					{
-						float f[N];
-						piece<T>::unpack(v[j], f);
-						#pragma unroll
-						for (int e = 0; e < N; ++e)
-							part.s += exp2_of((f[e] - base) * p.k);
-					}
-					part.s = vocab_warp_sum(part.s);
-
-					// every warp gets every warp's part, those of the cluster's other CTAs included
-					softmax_part * const slots = s_part[phase];
-					phase ^= 1;   // a slot is written again two exchanges later: one barrier in between is enough
-					if (split > 1)
-					{
-						if (lane < (int)split)
-							vocab_cluster_store(slots + rank * warps + warp, lane, part);
-						vocab_cluster_arrive();
-						vocab_cluster_wait();
-					}
-					else
-					{
-						if (lane == 0)
-							slots[warp] = part;
-						__syncthreads();
-					}
-					total.m = -INFINITY;
-					for (int i = lane; i < parts; i += 32)
-						total.m = fmaxf(total.m, slots[i].m);
-					total.m = vocab_warp_max(total.m);
-					for (int i = lane; i < parts; i += 32)
-						total.s += slots[i].s * rescale(slots[i].m, total.m, p.k);
-					total.s = vocab_warp_sum(total.s);
-					on = total.s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
-				}
-
-				// the row's loss, and what its probabilities are multiplied with
-				float c = 0.0F, at_token = 0.0F;
-				const bool first = rank == 0 && threadIdx.x == 0;
-				if (OP == kScore)
-				{
-					if (first)
-					{
-						p.logp[row] = on ? (xa - total.m) * p.inv_tau - logf(total.s) : 0.0F;
-						if (p.saved)
-						{
-							p.saved[row] = on ? total.m : 0.0F;
-							p.saved[p.rows + row] = on ? total.s : 0.0F;
-						}
-					}
-					continue;
-				}
-				const float weight = p.scale * w;
-				if (OP == kPolicy)
-				{
-					const policy_row l = policy_of(p, xa, total, weight, __ldg(p.old_logp + row), __ldg(p.advantages + row), p.ref_logp ? __ldg(p.ref_logp + row) : 0.0F, on);
-					c = l.c;
-					at_token = l.at_token;
-					if (first)
-					{
-						p.loss[row] = l.loss;
-						p.logp[row] = l.logp;
-						if (p.kl)
-							p.kl[row] = l.kl;
-					}
-					on = on && at_token != 0.0F | c != 0.0F;
-				}
-				if (OP == kDistill)
-				{
-					// the teacher's row is known to the first warp
-					if (rank == 0 && warp == 0)
-					{
-						float sum = 0.0F;
-						if (on && any && weight != 0.0F)
-						{
-							const float ln = logf(total.s);
-							for (int e = lane; e < p.kept; e += 32)
-								if (d.q[e] != 0.0F)
-									sum += d.q[e] * (d.lnq[e] - ((d.x[e] - total.m) * p.inv_tau - ln));
-							sum = vocab_warp_sum(sum) * (weight * p.tau * p.tau);
-						}
-						if (lane == 0)
-							p.loss[row] = sum;
-					}
-				}
-				if (!dx)
-				{
-					if (OP == kDistill)
-						__syncthreads();   // the teacher's row is read before the next one takes its place
-					continue;
-				}
-				if (OP == kDistill)
-				{
-					const bool valid = __syncthreads_or(any);
-					on = on && valid && weight != 0.0F;
-					c = on ? -weight * p.tau / total.s : 0.0F;
-				}
-				if (!on)
-				{
-					if (!p.add)
-						for (int i = from + (int)threadIdx.x; i < to; i += blockDim.x)
-							store_piece<T>(x, dx, aligned, i, 0, [](int) { return 0.0F; });
-					continue;
-				}
-				const int token_piece = OP == kPolicy ? (int)(token + x.shift) / N : -1, token_place = (int)(token + x.shift) % N;
-				#pragma unroll
-				for (int j = 0; j < NP; ++j)
-				{
-					const int i = from + j * (int)blockDim.x + (int)threadIdx.x;
-					if (i < to)
-					{
-						float f[N];
-						piece<T>::unpack(v[j], f);
-						#pragma unroll
-						for (int e = 0; e < N; ++e)
-							f[e] = exp2_of((f[e] - total.m) * p.k) * c;
-						if (OP == kPolicy && i == token_piece)
-						{
-							#pragma unroll
-							for (int e = 0; e < N; ++e)
-								f[e] = e == token_place ? at_token : f[e];
-						}
-						store_piece<T>(x, dx, aligned, i, p.add, [&](int e) { return f[e]; });
-					}
-				}
-				if (OP == kDistill)
-				{
-					// The columns that the teacher kept: c*(q - p), written over -c*p. An index that is there twice holds the sum of both; the
-					// first of its entries writes it. `seen` shows whether there is one at all.
-					bool twice = false;
-					for (int e = threadIdx.x; e < p.kept; e += blockDim.x)
-					{
-						const int col = d.id[e] < 0 ? -1 : d.id[e] + x.shift - from * N;
-						if (d.id[e] >= 0 && col >= 0 && col < (to - from) * N)
-						{
-							const uint32_t bit = 1u << (col & 31);
-							twice = twice || (atomicOr(d.seen + (col >> 5), bit) & bit);
-						}
-					}
-					twice = __syncthreads_or(twice);   // also: the pieces above are written
-					const float share = weight * p.tau;
-					for (int e = threadIdx.x; e < p.kept; e += blockDim.x)
-					{
-						const int id = d.id[e], col = id < 0 ? -1 : id + x.shift - from * N;
-						if (id >= 0 && col >= 0 && col < (to - from) * N)
-						{
-							d.seen[col >> 5] = 0;
-							float q = d.q[e];
-							bool leads = true;
-							if (twice)
-							{
-								q = 0.0F;
-								for (int o = 0; o < p.kept; ++o)
-									if (d.id[o] == id)
-									{
-										leads = leads && o >= e;
-										q += d.q[o];
-									}
-							}
-							if (leads)
-							{
-								const float g = exp2_of((d.x[e] - total.m) * p.k) * c + share * q;
-								piece<T>::store(dx + id, p.add ? d.old[e] + g : g);
-							}
-						}
-					}
-					__syncthreads();
-				}
-			}
-		}
 
 		constexpr unsigned long long kWaitNs = 5000000000ull;
 
@@ -939,12 +659,7 @@ namespace nnf
 				// the partial pieces, an element a thread
 				const int at = tid < N ? from : to - 1, e = tid % N;
 				if ((tid < N ? lo > from : hi < to) && x.has(at, e))
-				{
-					part.m = piece<T>::value(x.at + at * N - x.shift + e);
-					part.s = part.m == -INFINITY ? 0.0F : part.m - part.m + 1.0F;   // NaN stays
-					if (!(part.m == part.m))
-						part.m = -INFINITY;
-				}
+					part = part_of(piece<T>::value(x.at + at * N - x.shift + e));
 			}
 			for (int i = lo; i < hi; i += kScorePieces * step)
 			{
@@ -997,6 +712,385 @@ namespace nnf
 						p.saved[row] = on ? total.m : 0.0F;
 						p.saved[p.rows + row] = on ? total.s : 0.0F;
 					}
+				}
+			}
+		}
+
+		// The same for many rows: a warp takes row after row, and a row's first pieces are asked for while the one before it ends. Lane l
+		// keeps the token of the l-th of the warp's next 32 rows, so that rows that count for nothing cost no time.
+		constexpr int kRowWarps = 8;   // of a CTA
+
+		template <class T>
+		__global__ void __launch_bounds__(kRowWarps * 32, 4) vocab_score_warp_kernel(const vocab_params p)
+		{
+			constexpr int N = piece<T>::N, K = kScorePieces;
+			const int lane = (int)threadIdx.x & 31;
+			const int64_t warps = (int64_t)gridDim.x * kRowWarps;
+			const uint4 nothing = make_uint4(piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing);
+			pdl_begin();
+			int64_t begin = 0, end = p.rows;
+			if (p.offsets)
+				covered_rows(p, begin, end);
+			int64_t base = begin + (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5) - 32 * warps;   // the first of 32 rows, `warps` apart
+			uint32_t ahead = 0;          // those of them that count and are still to come
+			int token = 0;
+
+			// the row that comes next: its first pieces, its token's score, and of its partial pieces an element a lane
+			row_frame<T> x(nullptr, 0);
+			int64_t row = -1;
+			int lo = 0, hi = 0;
+			float xa = 0.0F, edge = -INFINITY;
+			uint4 next[K];
+			auto fetch = [&](int i)
+			{
+				#pragma unroll
+				for (int j = 0; j < K; ++j)
+				{
+					const int at = i + j * 32 + lane;
+					next[j] = at >= lo && at < hi ? __ldcs(x.address(at)) : nothing;
+				}
+			};
+			auto advance = [&]()
+			{
+				row = -1;
+				while (ahead == 0)
+				{
+					base += 32 * warps;
+					if (base >= end)
+						return;
+					const int64_t r = base + lane * warps;
+					const int64_t wide = r < end ? index_at(p.tokens, p.tokens_wide, r) : -1;
+					const bool on = wide >= 0 && wide < p.cols;
+					token = (int)wide;
+					if (!on && r < end)
+					{
+						p.logp[r] = 0.0F;
+						if (p.saved)
+							p.saved[r] = p.saved[p.rows + r] = 0.0F;
+					}
+					ahead = __ballot_sync(0xffffffffu, on);
+				}
+				const int l = __ffs((int)ahead) - 1;
+				ahead &= ahead - 1;
+				row = base + l * warps;
+				x = row_frame<T>(const_cast<T *>(static_cast<const T *>(p.x)) + row * p.ldx, p.cols);
+				lo = x.whole(0) ? 0 : 1;
+				hi = x.whole(x.pieces - 1) ? x.pieces : x.pieces - 1;
+				fetch(0);
+				xa = piece<T>::value(x.at + __shfl_sync(0xffffffffu, token, l));
+				if (lo > 0 || hi < x.pieces)
+					edge = edge_of(x, lane);
+			};
+			for (advance(); row >= 0;)
+			{
+				softmax_part part = {-INFINITY, 0.0F};
+				if (lo > 0 || hi < x.pieces)
+					part = part_of(edge);
+				uint4 v[K];
+				for (int i = K * 32; i < hi; i += K * 32)
+				{
+					#pragma unroll
+					for (int j = 0; j < K; ++j)
+						v[j] = next[j];
+					fetch(i);
+					add_part<T, K>(part, v, p.k);
+				}
+				#pragma unroll
+				for (int j = 0; j < K; ++j)
+					v[j] = next[j];
+				const int64_t done = row;
+				const float its_xa = xa;
+				advance();
+				add_part<T, K>(part, v, p.k);
+				const float m = vocab_warp_max(part.m);
+				const float s = vocab_warp_sum(part.s * rescale(part.m, m, p.k));
+				if (lane == 0)
+				{
+					const bool on = s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
+					p.logp[done] = on ? (its_xa - m) * p.inv_tau - logf(s) : 0.0F;
+					if (p.saved)
+					{
+						p.saved[done] = on ? m : 0.0F;
+						p.saved[p.rows + done] = on ? s : 0.0F;
+					}
+				}
+			}
+		}
+
+		// ---- short rows, with their gradient: a warp has a row in registers ---------------------------------------------------
+		// As above a warp takes row after row, and asks for the next one before it works on the one it has. NP: pieces of a lane.
+		template <class T, int OP, int NP, bool ANY>
+		__global__ void __launch_bounds__(kRowWarps * 32, NP > 4 ? 2 : 3) vocab_short_kernel(const vocab_params p)
+		{
+			constexpr int N = piece<T>::N;
+			extern __shared__ __align__(16) unsigned char s_short[];
+			const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
+			const int64_t warps = (int64_t)gridDim.x * kRowWarps;
+			const uint4 nothing = make_uint4(piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing);
+			distill_shared d = {};
+			if (OP == kDistill)
+			{
+				constexpr int words = NP * 32 * N / 32 + 1;
+				d.id = reinterpret_cast<int *>(s_short) + (size_t)warp * (4 * p.kept + words);
+				d.q = reinterpret_cast<float *>(d.id + p.kept);
+				d.x = d.q + p.kept;
+				d.old = d.x + p.kept;
+				d.seen = reinterpret_cast<uint32_t *>(d.old + p.kept);
+				for (int i = lane; i < words; i += 32)
+					d.seen[i] = 0;
+			}
+			pdl_begin();
+			int64_t base = (int64_t)blockIdx.x * kRowWarps + warp - 32 * warps;   // the first of 32 rows, `warps` apart
+			uint32_t ahead = 0;          // those of them that count and are still to come
+			int token = 0;               // of the lane's row, as the following
+			float weight = 0.0F, old_logp = 0.0F, advantage = 0.0F, ref_logp = 0.0F;
+
+			row_frame<T> x(nullptr, 0);  // the row that comes next
+			int64_t row = -1;
+			float xa = 0.0F, edge = -INFINITY, its_weight = 0.0F, its_old = 0.0F, its_advantage = 0.0F, its_ref = 0.0F;
+			int its_token = 0;
+			uint4 next[NP];
+			auto empty_row = [&](int64_t r)   // its gradient is nothing
+			{
+				const row_frame<T> e(const_cast<T *>(static_cast<const T *>(p.x)) + r * p.ldx, p.cols);
+				T * const dx = static_cast<T *>(p.dx) + r * p.lddx;
+				for (int i = lane; i < e.pieces; i += 32)
+					store_piece<T>(e, dx, !ANY, i, 0, [](int) { return 0.0F; });
+			};
+			auto advance = [&]()
+			{
+				row = -1;
+				while (ahead == 0)
+				{
+					base += 32 * warps;
+					if (base >= p.rows)
+						return;
+					const int64_t r = base + lane * warps;
+					const bool there = r < p.rows;
+					const float w = !there ? 0.0F : p.mask ? __ldg(p.mask + r) : 1.0F;
+					bool on = w != 0.0F;
+					weight = p.scale * w;
+					if (OP == kPolicy && there)
+					{
+						const int64_t wide = index_at(p.tokens, p.tokens_wide, r);
+						on = on && wide >= 0 && wide < p.cols;
+						token = (int)wide;
+						old_logp = __ldg(p.old_logp + r);
+						advantage = __ldg(p.advantages + r);
+						ref_logp = p.ref_logp ? __ldg(p.ref_logp + r) : 0.0F;
+					}
+					if (!on && there)
+					{
+						p.loss[r] = 0.0F;
+						if (OP == kPolicy)
+						{
+							p.logp[r] = 0.0F;
+							if (p.kl)
+								p.kl[r] = 0.0F;
+						}
+					}
+					ahead = __ballot_sync(0xffffffffu, on);
+					if (p.dx && !p.add)
+						for (uint32_t off = __ballot_sync(0xffffffffu, !on && there); off; off &= off - 1)
+							empty_row(base + (__ffs((int)off) - 1) * warps);
+				}
+				const int l = __ffs((int)ahead) - 1;
+				ahead &= ahead - 1;
+				row = base + l * warps;
+				x = row_frame<T>(const_cast<T *>(static_cast<const T *>(p.x)) + row * p.ldx, p.cols);
+				const int lo = x.whole(0) ? 0 : 1, hi = x.whole(x.pieces - 1) ? x.pieces : x.pieces - 1;
+				#pragma unroll
+				for (int j = 0; j < NP; ++j)
+				{
+					const int at = j * 32 + lane;
+					next[j] = at >= lo && at < hi ? __ldcs(x.address(at)) : nothing;
+				}
+				its_weight = __shfl_sync(0xffffffffu, weight, l);
+				if (OP == kPolicy)
+				{
+					its_token = __shfl_sync(0xffffffffu, token, l);
+					xa = piece<T>::value(x.at + its_token);
+					its_old = __shfl_sync(0xffffffffu, old_logp, l);
+					its_advantage = __shfl_sync(0xffffffffu, advantage, l);
+					its_ref = __shfl_sync(0xffffffffu, ref_logp, l);
+				}
+				edge = edge_of(x, lane);
+			};
+			for (advance(); row >= 0;)
+			{
+				const row_frame<T> y = x;
+				const int64_t done = row;
+				const float w = its_weight, at_edge = edge, score = xa, o = its_old, a = its_advantage, f = its_ref;
+				const int tok = its_token;
+				uint4 v[NP];
+				#pragma unroll
+				for (int j = 0; j < NP; ++j)
+					v[j] = next[j];
+				T * const dx = p.dx ? static_cast<T *>(p.dx) + done * p.lddx : nullptr;
+				float t_max = 0.0F, t_sum = 0.0F;
+				if (OP == kDistill)
+				{
+					float m = -INFINITY;
+					for (int e = lane; e < p.kept; e += 32)
+					{
+						const int64_t id = index_at(p.ids, p.ids_wide, done * p.ld_ids + e);
+						const bool in = id >= 0 && id < p.cols;
+						const float t = in ? value_at(p.teacher, p.teacher_type, done * p.ld_teacher + e) : -INFINITY;
+						d.id[e] = in ? (int)id : -1;
+						d.q[e] = t;
+						d.x[e] = in ? piece<T>::value(y.at + id) : 0.0F;
+						if (ANY && p.add && in)
+							d.old[e] = piece<T>::value(dx + id);
+						m = fmaxf(m, t);
+					}
+					m = vocab_warp_max(m);
+					t_max = m == -INFINITY ? 0.0F : m;
+					for (int e = lane; e < p.kept; e += 32)
+						t_sum += exp2_of((d.q[e] - t_max) * p.k);
+					t_sum = vocab_warp_sum(t_sum);
+				}
+				advance();
+
+				softmax_part total;
+				total.m = vocab_warp_max(fmaxf(piece<T>::template maximum<NP>(v), at_edge));
+				total.s = vocab_warp_sum(sum_of_exp<T, NP>(v, total.m, p.k) + (at_edge == -INFINITY ? 0.0F : exp2_of((at_edge - total.m) * p.k)));
+				bool on = total.s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
+				float c = 0.0F, at_token = 0.0F;
+				if (OP == kPolicy)
+				{
+					const policy_row l = policy_of(p, score, total, w, o, a, f, on);
+					c = l.c;
+					at_token = l.at_token;
+					if (lane == 0)
+					{
+						p.loss[done] = l.loss;
+						p.logp[done] = l.logp;
+						if (p.kl)
+							p.kl[done] = l.kl;
+					}
+					on = c != 0.0F || at_token != 0.0F;
+				}
+				else
+				{
+					on = on && t_sum != 0.0F && w != 0.0F;
+					c = on ? -w * p.tau / total.s : 0.0F;
+					float sum = 0.0F;
+					if (on)
+					{
+						const float ln = logf(total.s), t_ln = logf(t_sum);
+						for (int e = lane; e < p.kept; e += 32)
+						{
+							const float q = exp2_of((d.q[e] - t_max) * p.k);
+							if (q != 0.0F)
+								sum += q * (((d.q[e] - t_max) * p.inv_tau - t_ln) - ((d.x[e] - total.m) * p.inv_tau - ln));
+						}
+						sum = vocab_warp_sum(sum) * (w * p.tau * p.tau / t_sum);
+					}
+					if (lane == 0)
+						p.loss[done] = sum;
+				}
+				if (!dx)
+				{
+					__syncwarp();
+					continue;
+				}
+				if (!on)
+				{
+					if (!p.add)
+						empty_row(done);
+					__syncwarp();
+					continue;
+				}
+				const int lo = y.whole(0) ? 0 : 1, hi = y.whole(y.pieces - 1) ? y.pieces : y.pieces - 1;
+				const row_gradient<T> gradient(total.m, p.k, c);
+				if (ANY)
+				{
+					#pragma unroll
+					for (int j = 0; j < NP; ++j)
+					{
+						const int at = j * 32 + lane;
+						if (at >= lo && at < hi)
+						{
+							float g[N];
+							piece<T>::unpack(v[j], g);
+							#pragma unroll
+							for (int e = 0; e < N; ++e)
+							{
+								const int col = at * N - y.shift + e;
+								const float t = OP == kPolicy && col == tok ? at_token : exp2_of((g[e] - total.m) * p.k) * c;
+								piece<T>::store(dx + col, p.add ? piece<T>::value(dx + col) + t : t);
+							}
+						}
+					}
+				}
+				else
+				{
+					uint4 * const out = reinterpret_cast<uint4 *>(dx - y.shift);
+					if (gradient.near())
+					{
+						#pragma unroll
+						for (int j = 0; j < NP; ++j)
+							if (j * 32 + lane >= lo && j * 32 + lane < hi)
+								__stcs(out + j * 32 + lane, gradient.template whole<true>(v[j]));
+					}
+					else
+					{
+						#pragma unroll
+						for (int j = 0; j < NP; ++j)
+							if (j * 32 + lane >= lo && j * 32 + lane < hi)
+								__stcs(out + j * 32 + lane, gradient.template whole<false>(v[j]));
+					}
+				}
+				if (lo > 0 || hi < y.pieces)
+				{
+					const int at = lane < 16 ? 0 : y.pieces - 1, e = lane & 15, col = at * N - y.shift + e;
+					if (e < N && !y.whole(at) && (lane < 16 || y.pieces > 1) && y.has(at, e))
+					{
+						const float t = ANY && OP == kPolicy && col == tok ? at_token : exp2_of((at_edge - total.m) * p.k) * c;
+						piece<T>::store(dx + col, p.add ? piece<T>::value(dx + col) + t : t);
+					}
+				}
+				__syncwarp();   // what lies under the target's columns is written
+				if (!ANY && OP == kPolicy && lane == 0)
+					piece<T>::store(dx + tok, at_token);
+				if (OP == kDistill)
+				{
+					// the columns that the teacher kept, as in the kernel for long rows
+					bool twice = false;
+					for (int e = lane; e < p.kept; e += 32)
+						if (d.id[e] >= 0)
+						{
+							const uint32_t bit = 1u << (d.id[e] & 31);
+							twice = twice || (atomicOr(d.seen + (d.id[e] >> 5), bit) & bit);
+						}
+					twice = __any_sync(0xffffffffu, twice);
+					__syncwarp();
+					const float share = w * p.tau / t_sum;
+					for (int e = lane; e < p.kept; e += 32)
+					{
+						const int id = d.id[e];
+						if (id < 0)
+							continue;
+						d.seen[id >> 5] = 0;
+						float q = exp2_of((d.q[e] - t_max) * p.k);
+						bool leads = true;
+						if (twice)
+						{
+							q = 0.0F;
+							for (int i = 0; i < p.kept; ++i)
+								if (d.id[i] == id)
+								{
+									leads = leads && i >= e;
+									q += exp2_of((d.q[i] - t_max) * p.k);
+								}
+						}
+						if (leads)
+						{
+							const float g = exp2_of((d.x[e] - total.m) * p.k) * c + share * q;
+							piece<T>::store(dx + id, ANY && p.add ? d.old[e] + g : g);
+						}
+					}
+					__syncwarp();
 				}
 			}
 		}
@@ -1242,7 +1336,7 @@ namespace nnf
 				return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: temperature %g", who, (double)temperature);
 			// a row's frame may hold a piece more than its elements fill
 			const int64_t n = 16 / element_size(x->type);
-			if ((x->cols + 2 * n - 2) / n > int64_t(kVocabCluster) * kVocabThreads * kVocabPieces)
+			if ((x->cols + 2 * n - 2) / n > kMaxPieces)
 				return set_error(NNF_ERR_UNSUPPORTED, "%s: rows of %lld scores: at most 1 MiB a row", who, (long long)x->cols);
 			if (dx)
 			{
@@ -1307,54 +1401,57 @@ namespace nnf
 			return launch_rows(kernel, v.rows * cluster, threads, smem, (int)cluster, s, p);
 		}
 
+		template <class T>
+		int run_score(cudaStream_t s, vocab_params& p, int64_t pieces)
+		{
+			const int64_t slots = (int64_t)sm_count() * 4 * kRowWarps;
+			// warps: what the last turn of all of them leaves unused; CTAs: about 1.5 ns a row that starting and ending each costs
+			const int64_t idle = (div_up(p.rows, slots) * slots - p.rows) * pieces * 16 / 6500, turnover = p.rows * 3 / 2;
+			if (tune().vocab_form == 3 || (tune().vocab_form == 0 && idle < turnover))
+			{
+				const int64_t needed = div_up(p.rows, kRowWarps);
+				launch(vocab_score_warp_kernel<T>, needed < slots / kRowWarps ? needed : slots / kRowWarps, kRowWarps * 32, 0, s, p);
+				return check_launch("vocab_score_warp_kernel");
+			}
+			int64_t cluster = 1;
+			while (cluster < kVocabCluster && p.rows * cluster < 2 * sm_count() && pieces > cluster * 512)
+				cluster *= 2;
+			if (tune().vocab_split > 0)
+				cluster = tune().vocab_split;
+			p.cluster = (int)cluster;
+			int threads = (int)(div_up(div_up(div_up(pieces, cluster), 8), 32) * 32);
+			threads = threads > kScoreThreads ? kScoreThreads : threads;
+			return launch_rows(vocab_score_kernel<T>, p.rows * cluster, threads, 0, (int)cluster, s, p);
+		}
+
+		template <class T, int OP, int NP>
+		int run_short(cudaStream_t s, vocab_params& p)
+		{
+			const bool any = !p.dx || p.add || ((reinterpret_cast<uintptr_t>(p.dx) ^ reinterpret_cast<uintptr_t>(p.x)) & 15) != 0 ||
+				(p.rows > 1 && (p.lddx - p.ldx) * (int64_t)sizeof(T) % 16 != 0);
+			auto kernel = any ? vocab_short_kernel<T, OP, NP, true> : vocab_short_kernel<T, OP, NP, false>;
+			const size_t smem = OP == kDistill ? size_t(kRowWarps) * 4 * (4 * size_t(p.kept) + NP * piece<T>::N + 1) : 0;
+			const int limit = running_config().max_shared_memory_per_block_optin - 4096;
+			const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
+			if (e != cudaSuccess)
+				return set_error(NNF_ERR_CUDA, "vocab_short_kernel: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+			const int64_t needed = div_up(p.rows, kRowWarps), resident = (int64_t)sm_count() * (NP > 4 ? 2 : 3);
+			launch(kernel, needed < resident ? needed : resident, kRowWarps * 32, smem, s, p);
+			return check_launch("vocab_short_kernel");
+		}
+
 		template <class T, int OP>
 		int run_rows_of(cudaStream_t s, vocab_params& p)
 		{
-			if constexpr (OP == kScore)
-			{
-				if (tune().vocab_form != 1)
-				{
-					const int64_t pieces = (p.cols + 2 * int64_t(piece<T>::N) - 2) / piece<T>::N;
-					int64_t cluster = 1;
-					while (cluster < kVocabCluster && p.rows * cluster < 2 * sm_count() && pieces > cluster * 512)
-						cluster *= 2;
-					if (tune().vocab_split > 0)
-						cluster = tune().vocab_split;
-					const int64_t per = div_up(pieces, cluster);
-					int threads = (int)(div_up(div_up(per, 8), 32) * 32);
-					threads = threads < 32 ? 32 : threads > kScoreThreads ? kScoreThreads : threads;
-					p.cluster = (int)cluster;
-					return launch_rows(vocab_score_kernel<T>, p.rows * cluster, threads, 0, (int)cluster, s, p);
-				}
-			}
-			else
-			{
-				const int64_t pieces = (p.cols + 2 * int64_t(piece<T>::N) - 2) / piece<T>::N;
-				if (tune().vocab_form == 2 || (tune().vocab_form != 1 && pieces > 256))
-					return run_held<T, OP>(s, p, pieces);
-			}
 			constexpr int64_t n = piece<T>::N;
 			const int64_t pieces = (p.cols + 2 * n - 2) / n;
-			int64_t cluster = 1;
-			while (cluster < kVocabCluster && pieces > cluster * 512 * kVocabPieces)
-				cluster *= 2;
-			while (cluster < kVocabCluster && p.rows * cluster < sm_count() && pieces > cluster * 512)
-				cluster *= 2;
-			const int64_t per = div_up(pieces, cluster);
-			const int np = per <= 32 ? 1 : per <= 64 ? 2 : per <= 128 ? 4 : 8;
-			const int threads = (int)(div_up(div_up(per, np), 32) * 32);
-			p.cluster = (int)cluster;
-			size_t smem = 0;
-			if (OP == kDistill)
-				smem = size_t(p.kept) * 20 + size_t(div_up(np * threads * n, 32)) * 4;
-			const int64_t most = (int64_t(1) << 30) / cluster;
-			const int64_t grid = (p.rows < most ? p.rows : most) * cluster;
-			switch (np)
+			if constexpr (OP == kScore)
+				return run_score<T>(s, p, pieces);
+			else
 			{
-			case 1: return launch_rows(vocab_rows_kernel<T, OP, 1>, grid, threads, smem, (int)cluster, s, p);
-			case 2: return launch_rows(vocab_rows_kernel<T, OP, 2>, grid, threads, smem, (int)cluster, s, p);
-			case 4: return launch_rows(vocab_rows_kernel<T, OP, 4>, grid, threads, smem, (int)cluster, s, p);
-			default: return launch_rows(vocab_rows_kernel<T, OP, 8>, grid, threads, smem, (int)cluster, s, p);
+				if (pieces > 256 || tune().vocab_form == 2)
+					return run_held<T, OP>(s, p, pieces);
+				return pieces <= 32 ? run_short<T, OP, 1>(s, p) : pieces <= 64 ? run_short<T, OP, 2>(s, p) : pieces <= 128 ? run_short<T, OP, 4>(s, p) : run_short<T, OP, 8>(s, p);
 			}
 		}
 

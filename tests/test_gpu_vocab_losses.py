@@ -22,10 +22,10 @@ def capi():
     return capi
 
 
-@pytest.fixture(autouse=True, params=["built-in choice", "registers", "shared memory", "shared memory, split"])
+@pytest.fixture(autouse=True, params=["built-in choice", "shared memory", "shared memory, split", "warps"])
 def form(request, capi):
     """Every test runs in each form of the kernels, whatever the sizes for which it is chosen."""
-    capi.set_tuning("vocab_form", {"b": 0, "r": 1, "s": 2}[request.param[0]])
+    capi.set_tuning("vocab_form", {"b": 0, "s": 2, "w": 3}[request.param[0]])
     capi.set_tuning("vocab_split", 4 if "split" in request.param else 0)
     yield
     assert capi.fused_error_check() == 0
