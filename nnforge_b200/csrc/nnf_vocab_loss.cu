@@ -235,7 +235,7 @@ namespace nnf
 
 		struct held_result             // what the row comes to, found by the first warp
 		{
-			float m, c, at_token, share;
+			float m, s, c, at_token, share;
 			int on;
 		};
 
@@ -455,7 +455,7 @@ namespace nnf
 					total.s += s_part[i].s * rescale(s_part[i].m, total.m, p.k);
 				total.s = vocab_warp_sum(total.s);
 				on = total.s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
-				held_result r = {total.m, 0.0F, 0.0F, 0.0F, on};
+				held_result r = {total.m, total.s, 0.0F, 0.0F, 0.0F, on};
 				if (OP == kPolicy)
 				{
 					const policy_row l = policy_of(p, xa, total, weight, __ldg(p.old_logp + row), __ldg(p.advantages + row), p.ref_logp ? __ldg(p.ref_logp + row) : 0.0F, on);
@@ -476,32 +476,33 @@ namespace nnf
 					r.on = on;
 					r.c = on ? -weight * p.tau / total.s : 0.0F;
 					r.share = on ? weight * p.tau / t_sum : 0.0F;
-					if (rank == 0)
-					{
-						float sum = 0.0F;
-						if (on)
-						{
-							const float ln = logf(total.s), t_ln = logf(t_sum);
-							for (int e = lane; e < p.kept; e += 32)
-							{
-								const float q = exp2_of((d.q[e] - t_max) * p.k);
-								if (q != 0.0F)
-								{
-									const float xe = present(d.id[e]) ? piece<T>::value(held_at + place(d.id[e])) : d.x[e];
-									sum += q * (((d.q[e] - t_max) * p.inv_tau - t_ln) - ((xe - total.m) * p.inv_tau - ln));
-								}
-							}
-							sum = vocab_warp_sum(sum) * (weight * p.tau * p.tau / t_sum);
-						}
-						if (lane == 0)
-							p.loss[row] = sum;
-					}
 				}
 				if (lane == 0)
 					s_result = r;
 			}
 			__syncthreads();
 			const held_result r = s_result;
+			if (OP == kDistill && rank == 0 && warp == warps - 1)
+			{
+				// the loss, while the other warps are at the gradient
+				float sum = 0.0F;
+				if (r.on)
+				{
+					const float ln = logf(r.s), t_ln = logf(t_sum);
+					for (int e = lane; e < p.kept; e += 32)
+					{
+						const float q = exp2_of((d.q[e] - t_max) * p.k);
+						if (q != 0.0F)
+						{
+							const float xe = present(d.id[e]) ? piece<T>::value(held_at + place(d.id[e])) : d.x[e];
+							sum += q * (((d.q[e] - t_max) * p.inv_tau - t_ln) - ((xe - r.m) * p.inv_tau - ln));
+						}
+					}
+					sum = vocab_warp_sum(sum) * (weight * p.tau * p.tau / t_sum);
+				}
+				if (lane == 0)
+					p.loss[row] = sum;
+			}
 			if (!dx)
 				return;
 			if (!r.on)
