@@ -362,11 +362,9 @@ namespace nnf
 			{
 				d.id = reinterpret_cast<int *>(held + hp.slots);
 				d.q = reinterpret_cast<float *>(d.id + p.kept);
-				d.old = d.q + p.kept;
-				d.x = d.old + p.kept;
+				d.x = d.q + p.kept;
 				d.seen = reinterpret_cast<uint32_t *>(d.x + p.kept);
-				for (int i = tid; i < (count * N + 31) / 32; i += step)
-					d.seen[i] = 0;
+				d.old = reinterpret_cast<float *>(d.seen + (per * N + 31) / 32);   // kAnyRow
 				// the teacher's row, while the student's is on its way
 				float m = -INFINITY;
 				for (int e = tid; e < p.kept; e += step)
@@ -379,6 +377,8 @@ namespace nnf
 					d.q[e] = t;
 					if (in && (mine || rank == 0) && !present((int)id))
 						d.x[e] = piece<T>::value(x.at + id);   // (the first CTA finds the loss)
+					if (mine)
+						d.seen[((int)id - begin) >> 5] = 0;
 					if (ROW == kAnyRow && p.add && mine)
 						d.old[e] = piece<T>::value(dx + id);
 					m = fmaxf(m, t);
@@ -1390,7 +1390,7 @@ namespace nnf
 				(v.rows < 2 || (v.lddx - v.ldx) * (int64_t)sizeof(T) % 16 == 0);
 			const bool registers = aligned && threads == kHeldThreads && per >= 3 * chunk && tune().vocab_regs != 99;
 			p.slots = (int)((per - (registers ? chunk : 0) + 7) & ~int64_t(7));
-			const size_t smem = size_t(p.slots) * 16 + (OP == kDistill ? size_t(v.kept) * 16 + size_t(div_up(per * piece<T>::N, 32)) * 4 : 0);
+			const size_t smem = size_t(p.slots) * 16 + (OP == kDistill ? size_t(v.kept) * (aligned ? 12 : 16) + size_t(div_up(per * piece<T>::N, 32)) * 4 : 0);
 			auto kernel = registers ? vocab_held_kernel<T, OP, kRegisterRow> : aligned ? vocab_held_kernel<T, OP, kAlignedRow> : vocab_held_kernel<T, OP, kAnyRow>;
 			const int limit = running_config().max_shared_memory_per_block_optin - 4096;
 			if (smem > (size_t)limit)
