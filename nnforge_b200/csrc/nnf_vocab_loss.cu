@@ -748,7 +748,7 @@ namespace nnf
 				for (int j = 0; j < K; ++j)
 				{
 					const int at = i + j * 32 + lane;
-					next[j] = at >= lo && at < hi ? __ldcs(x.address(at)) : nothing;
+					next[j] = at >= lo && at < hi ? __ldg(x.address(at)) : nothing;
 				}
 			};
 			auto advance = [&]()
@@ -1117,12 +1117,14 @@ namespace nnf
 
 		constexpr int kBwdThreads = 256, kBwdPieces = 4;
 
-		template <class T>
+		// ALIGNED: whole pieces are stored at once (the gradient is not added, and its rows start where the logits' do in their 16 bytes).
+		// The last row comes first: the end of the logits is what the forward pass before has left in L2.
+		template <class T, bool ALIGNED>
 		__global__ void __launch_bounds__(kBwdThreads) vocab_bwd_kernel(const vocab_bwd_params p)
 		{
 			constexpr int N = piece<T>::N;
 			pdl_begin();
-			const int64_t row = blockIdx.x / p.slices;
+			const int64_t row = p.rows - 1 - blockIdx.x / p.slices;
 			if (p.offsets)
 			{
 				vocab_params q = {};
@@ -1134,50 +1136,56 @@ namespace nnf
 			}
 			const row_frame<T> x(const_cast<T *>(static_cast<const T *>(p.x)) + row * p.ldx, p.cols);
 			T * const dx = static_cast<T *>(p.dx) + row * p.lddx;
-			const bool aligned = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x.at)) & 15) == 0;
 			const int64_t token = index_at(p.tokens, p.tokens_wide, row);
 			const float g = __ldg(p.dlogp + row) * p.inv_tau, m = __ldg(p.saved + row), s = __ldg(p.saved + p.rows + row);
 			const bool on = token >= 0 && token < p.cols && s != 0.0F && g != 0.0F;
-			const int from = (int)(blockIdx.x % p.slices) * (int)(blockDim.x * kBwdPieces) + (int)threadIdx.x;
+			const int step = (int)blockDim.x, from = (int)(blockIdx.x % p.slices) * step * kBwdPieces + (int)threadIdx.x;
+			const int lo = x.whole(0) ? 0 : 1, hi = x.pieces > lo && !x.whole(x.pieces - 1) ? x.pieces - 1 : x.pieces;   // whole pieces
 			if (!on)
 			{
 				if (!p.add)
-					for (int j = 0, i = from; j < kBwdPieces && i < x.pieces; ++j, i += blockDim.x)
-						store_piece<T>(x, dx, aligned, i, 0, [](int) { return 0.0F; });
+					for (int j = 0, i = from; j < kBwdPieces && i < x.pieces; ++j, i += step)
+						store_piece<T>(x, dx, ALIGNED, i, 0, [](int) { return 0.0F; });
 				return;
 			}
-			const float c = -g / s;
-			const int token_piece = (int)(token + x.shift) / N, token_place = (int)(token + x.shift) % N;
-			uint4 v[kBwdPieces];
-			#pragma unroll
-			for (int j = 0; j < kBwdPieces; ++j)
-				if (from + j * (int)blockDim.x < x.pieces)
-					v[j] = x.load(from + j * (int)blockDim.x);
-			#pragma unroll
-			for (int j = 0; j < kBwdPieces; ++j)
+			const row_gradient<T> gradient(m, p.k, -g / s);
+			auto at = [&](int col)   // one element
 			{
-				const int i = from + j * (int)blockDim.x;
-				if (i < x.pieces)
-				{
-					float f[N];
-					piece<T>::unpack(v[j], f);
-					float at_token = 0.0F;
-					if (i == token_piece)
-					{
-						#pragma unroll
+				const float score = piece<T>::value(x.at + col);
+				const float t = col == (int)token ? -g * expm1f((score - m) * p.inv_tau - logf(s)) : exp2_of((score - m) * p.k) * gradient.c;
+				return p.add ? piece<T>::value(dx + col) + t : t;
+			};
+			if (ALIGNED && gradient.near())
+			{
+				uint4 v[kBwdPieces];
+				#pragma unroll
+				for (int j = 0; j < kBwdPieces; ++j)
+					if (from + j * step >= lo && from + j * step < hi)
+						v[j] = __ldcs(x.address(from + j * step));
+				float at_token = 0.0F;
+				const int token_piece = (int)(token + x.shift) / N;
+				const bool mine = token_piece >= from && token_piece < from + kBwdPieces * step && (token_piece - from) % step == 0;
+				if (mine)
+					at_token = at((int)token);   // before it is written over, should the gradient take the scores' place
+				uint4 * const out = reinterpret_cast<uint4 *>(dx - x.shift);
+				#pragma unroll
+				for (int j = 0; j < kBwdPieces; ++j)
+					if (from + j * step >= lo && from + j * step < hi)
+						__stcs(out + from + j * step, gradient.template whole<true>(v[j]));
+				if (mine && token_piece >= lo && token_piece < hi)
+					piece<T>::store(dx + token, at_token);
+				for (int i = from, j = 0; j < kBwdPieces && i < x.pieces; ++j, i += step)
+					if (i < lo || i >= hi)
 						for (int e = 0; e < N; ++e)
-							at_token = e == token_place ? f[e] : at_token;
-						at_token = -g * expm1f((at_token - m) * p.inv_tau - logf(s));   // g * (1 - p)
-					}
-					#pragma unroll
-					for (int e = 0; e < N; ++e)
-					{
-						f[e] = exp2_of((f[e] - m) * p.k) * c;
-						if (i == token_piece && e == token_place)
-							f[e] = at_token;
-					}
-					store_piece<T>(x, dx, aligned, i, p.add, [&](int e) { return f[e]; });
-				}
+							if (x.has(i, e))
+								piece<T>::store(dx + i * N - x.shift + e, at(i * N - x.shift + e));
+			}
+			else
+			{
+				// element by element, a CTA's elements side by side
+				const int first = (from - (int)threadIdx.x) * N - x.shift, last = min(first + kBwdPieces * step * N, p.cols);
+				for (int col = max(first, 0) + (int)threadIdx.x; col < last; col += step)
+					piece<T>::store(dx + col, at(col));
 			}
 		}
 
@@ -1486,11 +1494,13 @@ namespace nnf
 			const int64_t grid = x.rows * p.slices;
 			if (grid > 0x7fffffff)
 				return set_error(NNF_ERR_UNSUPPORTED, "token log probabilities, backward: too many rows");
+			const bool aligned = !p.add && ((reinterpret_cast<uintptr_t>(dx.data) ^ reinterpret_cast<uintptr_t>(x.data)) & 15) == 0 &&
+				(x.rows < 2 || (dx.stride - x.stride) * element_size(x.type) % 16 == 0);
 			switch (x.type)
 			{
-			case NNF_F32: launch(vocab_bwd_kernel<float>, grid, threads, 0, s, p); break;
-			case NNF_BF16: launch(vocab_bwd_kernel<__nv_bfloat16>, grid, threads, 0, s, p); break;
-			default: launch(vocab_bwd_kernel<__half>, grid, threads, 0, s, p); break;
+			case NNF_F32: launch(aligned ? vocab_bwd_kernel<float, true> : vocab_bwd_kernel<float, false>, grid, threads, 0, s, p); break;
+			case NNF_BF16: launch(aligned ? vocab_bwd_kernel<__nv_bfloat16, true> : vocab_bwd_kernel<__nv_bfloat16, false>, grid, threads, 0, s, p); break;
+			default: launch(aligned ? vocab_bwd_kernel<__half, true> : vocab_bwd_kernel<__half, false>, grid, threads, 0, s, p); break;
 			}
 			return check_launch("vocab_bwd_kernel");
 		}
