@@ -345,4 +345,14 @@ namespace nnf
 		asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
 		asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" :: "r"(a), "f"(v.m), "f"(v.s) : "memory");
 	}
+
+	// the same, counted by a barrier of that CTA
+	__device__ __forceinline__ void vocab_cluster_send(const softmax_part * p, const uint64_t * bar, uint32_t rank, softmax_part v)
+	{
+		uint32_t a, b;
+		asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+		asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"((uint32_t)__cvta_generic_to_shared(bar)), "r"(rank));
+		asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];"
+			:: "r"(a), "f"(v.m), "f"(v.s), "r"(b) : "memory");
+	}
 }

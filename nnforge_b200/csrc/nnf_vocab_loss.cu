@@ -246,6 +246,7 @@ namespace nnf
 			extern __shared__ __align__(128) unsigned char s_held[];
 			__shared__ softmax_part s_part[kVocabCluster * (kHeldThreads / 32)];
 			__shared__ uint64_t s_bar[kHeldChunks];
+			__shared__ uint64_t s_exchanged;
 			__shared__ held_result s_result;
 			__shared__ float s_red[2][kHeldThreads / 32];
 			const vocab_params& p = hp.v;
@@ -254,7 +255,15 @@ namespace nnf
 			const int tid = (int)threadIdx.x, step = (int)blockDim.x, lane = tid & 31, warp = tid >> 5, warps = step >> 5;
 			const int64_t row = blockIdx.x / split;
 			if (split > 1)
+			{
+				if (tid == 0)
+				{
+					mbar_init(&s_exchanged, 1);
+					asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+					mbar_arrive_expect(&s_exchanged, split * (uint32_t)warps * (uint32_t)sizeof(softmax_part));
+				}
 				vocab_cluster_arrive();   // waited for before the first store into another CTA
+			}
 			const row_frame<T> x(const_cast<T *>(static_cast<const T *>(p.x)) + row * p.ldx, p.cols);
 			T * const dx = p.dx ? static_cast<T *>(p.dx) + row * p.lddx : nullptr;
 			const int per = split > 1 ? (x.pieces + (int)split - 1) / (int)split : x.pieces;
@@ -430,14 +439,14 @@ namespace nnf
 				part.s = vocab_warp_sum(part.s * rescale(part.m, m, p.k));
 				part.m = m;
 			}
-			// the first warp of every CTA gets every warp's part
+			// the first warp of every CTA gets every warp's part (and no CTA leaves before all have sent it theirs)
 			if (split > 1)
 			{
 				vocab_cluster_wait();
 				if (lane < (int)split)
-					vocab_cluster_store(s_part + rank * warps + warp, lane, part);
-				vocab_cluster_arrive();
-				vocab_cluster_wait();
+					vocab_cluster_send(s_part + rank * warps + warp, &s_exchanged, lane, part);
+				if (warp == 0)
+					mbar_wait(&s_exchanged, 0, gave_up, hp.error);
 			}
 			else
 			{
