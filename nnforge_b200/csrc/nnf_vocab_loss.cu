@@ -1393,6 +1393,9 @@ namespace nnf
 			int64_t cluster = 1;
 			while (cluster < kVocabCluster && pieces > cluster * 4200)
 				cluster *= 2;
+			// few rows: over more CTAs, as long as those are less than four an SM
+			while (cluster < kVocabCluster && v.rows * cluster * 2 < 4 * sm_count() && pieces > cluster * 512)
+				cluster *= 2;
 			if (tune().vocab_split > 0)
 				cluster = tune().vocab_split;
 			held_params p = {};
@@ -1400,7 +1403,8 @@ namespace nnf
 			p.v.cluster = (int)cluster;
 			p.error = device_error_word();
 			const int64_t per = div_up(pieces, cluster);
-			int threads = (int)(div_up(div_up(per, 16), 32) * 32);
+			// 16 pieces a thread; where the SMs are not full, four
+			int threads = (int)(div_up(div_up(per, v.rows * cluster < 4 * sm_count() ? 4 : 16), 32) * 32);
 			threads = threads < 64 ? 64 : threads > kHeldThreads ? kHeldThreads : threads;
 			const int64_t chunk = int64_t(threads) * kHeldChunk;
 			const bool aligned = v.dx && !v.add && ((reinterpret_cast<uintptr_t>(v.dx) ^ reinterpret_cast<uintptr_t>(v.x)) & 15) == 0 &&
