@@ -95,7 +95,7 @@ NNF_API int nnf_get_running_configuration(nnf_running_configuration * out);
 /* Knobs of the launch plans (process-wide; nothing in the library reads the environment). No counterpart in
  * the reference. name: "elementwise_waves", "elementwise_group_waves", "pool_waves", "pool_group_floats", "pool_staged",
  * "channel_waves", "group_waves", "chain_s_kb", "chain_a_kb", "chain_dist" (-1: built-in), "chain_chunk_mb",
- * "chain_lag" (lag + 1), "chain_cluster" (99: not that form), "vocab_form" (1: rows in registers, 2: rows in shared memory), "vocab_split" (CTAs of a row), "no_grouped", "apply_flat", "peer_wait_ns" (how long a batch-sharded launch waits for
+ * "chain_lag" (lag + 1), "chain_cluster" (99: not that form), "vocab_form" (2: a CTA per row, the row in shared memory; 3: scores by warps), "vocab_split" (CTAs of a row, at most 8), "no_grouped", "apply_flat", "peer_wait_ns" (how long a batch-sharded launch waits for
  * another rank's statistics before it gives up; default 10 s), or "reset" (all back to the built-in choices).
  * A value <= 0 selects the built-in choice. Meant for tests that walk the geometries and for tuning. */
 NNF_API int nnf_set_tuning(const char * name, long long value);

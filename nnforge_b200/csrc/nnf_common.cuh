@@ -101,8 +101,7 @@ namespace nnf
 		int chain_cluster;            // CTAs per channel of the cluster form (1, 2, 4, 8); 99: never that form
 		int no_grouped;               // 1: planes that are not whole float4s take the per-channel kernels
 		int apply_flat;               // 1: training apply through the flat streaming kernel
-		int vocab_form;               // losses on a vocabulary: 1 rows in registers, 2 rows in shared memory
-		int vocab_regs;
+		int vocab_form;               // losses on a vocabulary: 2 a CTA per row, the row in shared memory; 3 scores by warps
 		int vocab_split;              // CTAs of a row in those
 		long long peer_wait_ns;       // how long a launch waits for another rank's statistics before it gives up
 	};

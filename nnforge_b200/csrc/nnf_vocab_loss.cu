@@ -71,13 +71,15 @@ namespace nnf
 			return __ldg(static_cast<const float *>(p) + i);
 		}
 
+		__device__ __forceinline__ int64_t within(int64_t row, int64_t rows) { return row < 0 ? 0 : row > rows ? rows : row; }
+
 		// the rows that the packed sequences cover
 		__device__ __forceinline__ void covered_rows(const vocab_params& p, int64_t& begin, int64_t& end)
 		{
 			begin = index_at(p.offsets, p.offsets_wide, 0);
 			end = index_at(p.offsets, p.offsets_wide, p.sequences);
-			begin = begin < 0 ? 0 : begin;
-			end = end > p.rows ? p.rows : end;
+			begin = within(begin, p.rows);
+			end = within(end, p.rows);
 		}
 
 		// stores a piece of the gradient's row: whole and aligned pieces at once, others element by element
@@ -172,10 +174,6 @@ namespace nnf
 		__device__ __forceinline__ void mbar_init(uint64_t * b, int count)
 		{
 			asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(shared_address(b)), "r"(count) : "memory");
-		}
-		__device__ __forceinline__ void mbar_arrive(uint64_t * b)
-		{
-			asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(shared_address(b)) : "memory");
 		}
 		__device__ __forceinline__ void mbar_arrive_expect(uint64_t * b, uint32_t bytes)
 		{
@@ -733,7 +731,7 @@ namespace nnf
 		template <class T>
 		__global__ void __launch_bounds__(kRowWarps * 32, 4) vocab_score_warp_kernel(const vocab_params p)
 		{
-			constexpr int N = piece<T>::N, K = kScorePieces;
+			constexpr int K = kScorePieces;
 			const int lane = (int)threadIdx.x & 31;
 			const int64_t warps = (int64_t)gridDim.x * kRowWarps;
 			const uint4 nothing = make_uint4(piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing);
@@ -1122,6 +1120,7 @@ namespace nnf
 			int offsets_wide;
 			int64_t sequences;
 			int slices;                // CTAs of a row
+			int64_t last;              // the last row of this launch, which comes first
 		};
 
 		constexpr int kBwdThreads = 256, kBwdPieces = 4;
@@ -1133,7 +1132,7 @@ namespace nnf
 		{
 			constexpr int N = piece<T>::N;
 			pdl_begin();
-			const int64_t row = p.rows - 1 - blockIdx.x / p.slices;
+			const int64_t row = p.last - blockIdx.x / p.slices;
 			if (p.offsets)
 			{
 				vocab_params q = {};
@@ -1230,16 +1229,17 @@ namespace nnf
 			#pragma unroll
 			for (int side = 0; side < 2; ++side)
 			{
-				begin[side] = max(index_at(p.offsets, p.offsets_wide, 2 * pair + side), (int64_t)0);
-				end[side] = min(index_at(p.offsets, p.offsets_wide, 2 * pair + side + 1), p.rows);
+				begin[side] = within(index_at(p.offsets, p.offsets_wide, 2 * pair + side), p.rows);
+				end[side] = within(index_at(p.offsets, p.offsets_wide, 2 * pair + side + 1), p.rows);
 				double t = 0.0;
 				long long n = 0;
+				#pragma unroll 4
 				for (int64_t r = begin[side] + threadIdx.x; r < end[side]; r += kPairThreads)
-					if (p.saved[p.rows + r] != 0.0F)
-					{
-						t += (double)p.logp[r];
-						++n;
-					}
+				{
+					const float s = p.saved[p.rows + r], l = p.logp[r];
+					t += s != 0.0F ? (double)l : 0.0;
+					n += s != 0.0F;
+				}
 				#pragma unroll
 				for (int o = 16; o > 0; o >>= 1)
 				{
@@ -1294,6 +1294,7 @@ namespace nnf
 			for (int side = 0; side < 2; ++side)
 			{
 				const float g = (side == 0 ? -dh : dh) * p.scale * share[side];
+				#pragma unroll 4
 				for (int64_t r = begin[side] + threadIdx.x; r < end[side]; r += kPairThreads)
 					p.dlogp[r] = p.saved[p.rows + r] != 0.0F ? g : 0.0F;
 			}
@@ -1350,7 +1351,7 @@ namespace nnf
 				st = check_rows(who, "dlogits", dx, is_float);
 			if (st != NNF_OK)
 				return st;
-			if (!(temperature > 0.0F) || !(temperature < INFINITY))
+			if (!(temperature >= 1.1754944e-38F) || !(temperature < INFINITY))   // 1/temperature is finite
 				return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: temperature %g", who, (double)temperature);
 			// a row's frame may hold a piece more than its elements fill
 			const int64_t n = 16 / element_size(x->type);
@@ -1397,7 +1398,7 @@ namespace nnf
 			while (cluster < kVocabCluster && v.rows * cluster * 2 < 4 * sm_count() && pieces > cluster * 512)
 				cluster *= 2;
 			if (tune().vocab_split > 0)
-				cluster = tune().vocab_split;
+				cluster = tune().vocab_split < kVocabCluster ? tune().vocab_split : kVocabCluster;
 			held_params p = {};
 			p.v = v;
 			p.v.cluster = (int)cluster;
@@ -1409,7 +1410,7 @@ namespace nnf
 			const int64_t chunk = int64_t(threads) * kHeldChunk;
 			const bool aligned = v.dx && !v.add && ((reinterpret_cast<uintptr_t>(v.dx) ^ reinterpret_cast<uintptr_t>(v.x)) & 15) == 0 &&
 				(v.rows < 2 || (v.lddx - v.ldx) * (int64_t)sizeof(T) % 16 == 0);
-			const bool registers = aligned && threads == kHeldThreads && per >= 3 * chunk && tune().vocab_regs != 99;
+			const bool registers = aligned && threads == kHeldThreads && per >= 3 * chunk;
 			p.slots = (int)((per - (registers ? chunk : 0) + 7) & ~int64_t(7));
 			const size_t smem = size_t(p.slots) * 16 + (OP == kDistill ? size_t(v.kept) * (aligned ? 12 : 16) + size_t(div_up(per * piece<T>::N, 32)) * 4 : 0);
 			auto kernel = registers ? vocab_held_kernel<T, OP, kRegisterRow> : aligned ? vocab_held_kernel<T, OP, kAlignedRow> : vocab_held_kernel<T, OP, kAnyRow>;
@@ -1439,10 +1440,13 @@ namespace nnf
 			while (cluster < kVocabCluster && p.rows * cluster < 2 * sm_count() && pieces > cluster * 512)
 				cluster *= 2;
 			if (tune().vocab_split > 0)
-				cluster = tune().vocab_split;
+				cluster = tune().vocab_split < kVocabCluster ? tune().vocab_split : kVocabCluster;
 			p.cluster = (int)cluster;
 			int threads = (int)(div_up(div_up(div_up(pieces, cluster), 8), 32) * 32);
-			threads = threads > kScoreThreads ? kScoreThreads : threads;
+			// 128 threads a row: twice the rows of 256 are in flight, so that fewer of them are at their start or end (8192x32000 bf16 85.8
+			// against 90.7 us, 3000x50000 53.5 / 56.5); 256 where that leaves the last turn emptier (2048x131072 86 against 90 us, 300x65536 10.9 / 11.7)
+			const int most = p.rows < 4 * sm_count() || (pieces > 8192 && p.rows < 16 * sm_count()) ? kScoreThreads : kScoreThreads / 2;
+			threads = threads > most ? most : threads;
 			return launch_rows(vocab_score_kernel<T>, p.rows * cluster, threads, 0, (int)cluster, s, p);
 		}
 
@@ -1504,18 +1508,23 @@ namespace nnf
 			const int64_t n = 16 / element_size(x.type), pieces = (x.cols + 2 * n - 2) / n;
 			const int threads = pieces < kBwdThreads * kBwdPieces ? (int)div_up(div_up(pieces, kBwdPieces), 32) * 32 : kBwdThreads;
 			p.slices = (int)div_up(pieces, threads * kBwdPieces);
-			const int64_t grid = x.rows * p.slices;
-			if (grid > 0x7fffffff)
-				return set_error(NNF_ERR_UNSUPPORTED, "token log probabilities, backward: too many rows");
 			const bool aligned = !p.add && ((reinterpret_cast<uintptr_t>(dx.data) ^ reinterpret_cast<uintptr_t>(x.data)) & 15) == 0 &&
 				(x.rows < 2 || (dx.stride - x.stride) * element_size(x.type) % 16 == 0);
-			switch (x.type)
+			const int64_t most = 0x7fffffff / p.slices;   // rows of a launch
+			for (p.last = x.rows - 1; p.last >= 0; p.last -= most)
 			{
-			case NNF_F32: launch(aligned ? vocab_bwd_kernel<float, true> : vocab_bwd_kernel<float, false>, grid, threads, 0, s, p); break;
-			case NNF_BF16: launch(aligned ? vocab_bwd_kernel<__nv_bfloat16, true> : vocab_bwd_kernel<__nv_bfloat16, false>, grid, threads, 0, s, p); break;
-			default: launch(aligned ? vocab_bwd_kernel<__half, true> : vocab_bwd_kernel<__half, false>, grid, threads, 0, s, p); break;
+				const int64_t grid = (p.last + 1 < most ? p.last + 1 : most) * p.slices;
+				switch (x.type)
+				{
+				case NNF_F32: launch(aligned ? vocab_bwd_kernel<float, true> : vocab_bwd_kernel<float, false>, grid, threads, 0, s, p); break;
+				case NNF_BF16: launch(aligned ? vocab_bwd_kernel<__nv_bfloat16, true> : vocab_bwd_kernel<__nv_bfloat16, false>, grid, threads, 0, s, p); break;
+				default: launch(aligned ? vocab_bwd_kernel<__half, true> : vocab_bwd_kernel<__half, false>, grid, threads, 0, s, p); break;
+				}
+				const int st = check_launch("vocab_bwd_kernel");
+				if (st != NNF_OK)
+					return st;
 			}
-			return check_launch("vocab_bwd_kernel");
+			return NNF_OK;
 		}
 	}
 }

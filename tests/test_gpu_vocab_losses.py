@@ -614,3 +614,141 @@ def test_tensors_that_are_refused(capi):
         capi.preference_loss(full(2), full(4), v, saved, v, x, t, full(4, dtype=torch.int64), full(4))
     with pytest.raises(ValueError, match="rewards"):
         capi.preference_loss(full(2), full(3), v, saved, v, x, t, full(5, dtype=torch.int64), full(4))
+
+
+@pytest.mark.parametrize("dtype,spread,tau", [("fp32", 1e3, 1.0), ("fp32", 1e8, 7.0), ("fp32", 3.0, 1e-4), ("bf16", 300.0, 1.0), ("bf16", 1e7, 1.0), ("fp16", 1e4, 1.0),
+                                              ("fp16", 3.0, 0.003)])
+@pytest.mark.parametrize("cols", [100, 3001, 33000])
+def test_large_scores(capi, cols, dtype, spread, tau):
+    """Scores so far apart that a row's maximum has nearly all of the mass, and so large that x*k - M*k would lose it. With |x - M|/tau up to
+    T (of those that matter: 104, where exp() leaves fp32) the argument of an exponential is off by 3u*T = 312u, beside the 77u + 4u of the sum:
+    GRAD (500u) still holds for p; logp is off by 4u*|x_token - M|/tau + 400u."""
+    g = generator(cols)
+    rows = 6
+    x = scores(g, rows, cols, TYPES[dtype], spread=spread)
+    x = torch.where(torch.isfinite(x), x, torch.zeros_like(x))   # (fp16 ends at 65504)
+    tokens = x.float().argmax(dim=1)
+    tokens[0] = 1
+    up = torch.randn(rows, device="cuda", generator=g)
+    logp, loss = vectors(rows, 2)
+    saved = torch.empty(2, rows, device="cuda")
+    capi.token_logp_fwd(logp, saved, x, tokens, temperature=tau)
+    want, _, on, tol, p = exact.token_logp(x, tokens, tau)
+    exact.check(logp, want, tol + 400 * exact.U, "logp")
+    value, size = exact.gradient(p, tokens, on, up.double(), up.double().abs(), tau)
+    _, dx = room(rows, cols, TYPES[dtype])
+    capi.token_logp_bwd(dx, up, x, tokens, saved, temperature=tau)
+    exact.check(dx, value, exact.GRAD * size, "dlogits of logp")
+    ids = torch.stack([tokens, (tokens + 1) % cols, (tokens + 2) % cols], dim=1)
+    top = torch.tensor([[3.0, 2.0, -4.0]], device="cuda").repeat(rows, 1) * tau
+    for add in (False, True):
+        _, dx = room(rows, cols, TYPES[dtype], value=0.0)
+        capi.policy_loss(loss, logp, x, tokens, want.float().clamp(min=-50), torch.ones(rows, device="cuda"), dlogits=dx, clip_low=1.0, clip_high=10.0, temperature=tau,
+                         add_to_destination=add)
+        result = exact.policy(x, tokens, want.float().clamp(min=-50), torch.ones(rows, device="cuda"), None, None, 1.0, 10.0, 0.0, tau, 1.0)
+        exact.check(dx, result["dlogits"][0], 2 * result["dlogits"][1], "dlogits of the policy")
+        _, dx = room(rows, cols, TYPES[dtype], value=0.0)
+        capi.distill_topk_loss(loss, x, ids, top, dlogits=dx, temperature=tau, add_to_destination=add)
+        result = exact.distill(x, ids, top, None, tau, 1.0)
+        exact.check(loss, *result["loss"], "distillation")
+        exact.check(dx, *result["dlogits"], "dlogits of the distillation")
+
+
+@pytest.mark.parametrize("cols", [64, 2000, 33000])
+def test_teachers_of_every_kind(capi, cols):
+    """The type's lowest value among a teacher's logits, rows of nothing else, NaN and infinity in one row only, a student who excludes what
+    the teacher keeps."""
+    g = generator(cols + 1)
+    low = torch.finfo(torch.float32).min
+    x = scores(g, 6, cols, torch.float32)
+    ids = torch.rand(6, cols, device="cuda", generator=g).topk(5, dim=1).indices
+    top = torch.randn(6, 5, device="cuda", generator=g)
+    top[0, 2:] = low
+    top[1] = low
+    top[2, 1] = math.nan
+    top[3, 4] = math.inf
+    x[4, ids[4, 0]] = -math.inf
+    loss, = vectors(6, 1)
+    _, dx = room(6, cols, torch.float32)
+    capi.distill_topk_loss(loss, x, ids, top, dlogits=dx)
+    keep = torch.tensor([0, 1, 5], device="cuda")
+    want = exact.distill(x[keep], ids[keep], top[keep], None, 1.0, 1.0)
+    exact.check(loss[keep], *want["loss"], "loss")
+    exact.check(dx[keep], *want["dlogits"], "dlogits")
+    assert math.isnan(float(loss[2])) and math.isnan(float(loss[3])) and float(loss[4]) == math.inf
+    assert bool(torch.isfinite(dx[4]).all())
+    want = exact.distill(x[4:5], ids[4:5], top[4:5], None, 1.0, 1.0)
+    exact.check(dx[4:5], *want["dlogits"], "dlogits where the student excludes it")
+
+
+def test_offsets_at_the_ends_of_their_type(capi):
+    x = scores(generator(13), 9, 70, torch.float32)
+    tokens = somewhere(generator(13), 9, 70, out=False)
+    big = 2 ** 63 - 1
+    for offsets in ([-big - 1, 4, big], [big, big, big], [big, 3, 0], [-big, -big, -big], [big - 1, big, -1]):
+        logp, dlogp = vectors(9, 2)
+        backing = torch.full((11, 70), 7.0, device="cuda")
+        capi.preference_loss(torch.empty(1, device="cuda"), torch.empty(2, device="cuda"), logp, torch.zeros(2, 9, device="cuda"), dlogp, x, tokens,
+                             torch.tensor(offsets, device="cuda"), torch.zeros(2, device="cuda"), dlogits=backing[1:10])
+        torch.cuda.synchronize()
+        assert bool((backing[0] == 7.0).all()) and bool((backing[10] == 7.0).all())
+
+
+def test_a_pair_that_is_no_number_stays_alone(capi):
+    g = generator(14)
+    x = scores(g, 12, 500, torch.bfloat16)
+    x[4, 7] = math.nan
+    tokens = somewhere(g, 12, 500, out=False)
+    offsets = torch.tensor([0, 3, 6, 9, 12], device="cuda")
+    loss, rewards, logp, dlogp = torch.empty(2, device="cuda"), *vectors(4, 1), *vectors(12, 2)
+    _, dx = room(12, 500, torch.bfloat16)
+    capi.preference_loss(loss, rewards, logp, torch.empty(2, 12, device="cuda"), dlogp, x, tokens, offsets, torch.zeros(4, device="cuda"), dlogits=dx)
+    assert math.isnan(float(loss[0])) and math.isfinite(float(loss[1]))
+    assert bool(torch.isnan(dx[:6]).any()) and bool(torch.isfinite(dx[6:]).all())
+
+
+def test_two_calls_at_once(capi):
+    """Two streams with a step each, many times over, give what they give one after the other."""
+    steps = [step_of(capi, generator(30 + k), rows=200, cols=20000) for k in range(2)]
+    names = ("logp", "old", "ref", "loss", "dloss", "dx")
+    want = []
+    for s, step in steps:
+        step()
+        torch.cuda.synchronize()
+        want.append({n: s[n].clone() for n in names})
+    streams = [torch.cuda.Stream() for _ in steps]
+    for _ in range(10):
+        for (s, step), stream in zip(steps, streams):
+            with torch.cuda.stream(stream):
+                step()
+    torch.cuda.synchronize()
+    for (s, _), w in zip(steps, want):
+        assert all(torch.equal(s[n], w[n]) for n in names)
+
+
+def test_the_first_call_of_a_process_may_be_captured(form, capi, request):
+    import os
+    import subprocess
+    import sys
+    if "built-in" not in request.node.name:
+        pytest.skip("the same in every form")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch
+from nnforge_b200 import capi
+x = torch.randn(8, 20000, device="cuda").bfloat16()
+t = torch.arange(8, device="cuda")
+v = [torch.zeros(8, device="cuda") for _ in range(4)]
+dx = torch.empty_like(x)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    capi.policy_loss(v[0], v[1], x, t, v[2], v[3], dlogits=dx)
+graph.replay()
+torch.cuda.synchronize()
+got = v[1].clone()
+capi.policy_loss(v[0], v[1], x, t, v[2], v[3], dlogits=dx)
+assert torch.equal(got, v[1]) and float(got.abs().sum()) > 0
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]

@@ -54,7 +54,7 @@ def test_logits(call, bad, status, text):
     assert text in capi.last_error()
 
 
-@pytest.mark.parametrize("tau", [0.0, -1.0, float("nan"), float("inf")])
+@pytest.mark.parametrize("tau", [0.0, -1.0, float("nan"), float("inf"), 1e-38])
 def test_temperatures(tau):
     for status in (forward(matrix(), indices(), tau=tau), backward(matrix(), matrix(), tau=tau), policy(tau=tau), preference(tau=tau), distill(tau=tau)):
         assert status == INVALID and "temperature" in capi.last_error()
