@@ -204,14 +204,17 @@ namespace nnf
 
 	// What a part's exponentials are multiplied with when the maximum becomes m. A part without a maximum (-infinity) keeps its sum: 0, or
 	// NaN where an element was NaN, which no maximum shows.
-	__device__ __forceinline__ float rescale(float part_m, float m, float k)
+	__device__ __forceinline__ float rescale(float part_m, float m, float k, float rest = 0.0F)
 	{
-		return part_m == m ? 1.0F : exp2_of((part_m - m) * k);
+		const float gap = part_m - m;
+		return part_m == m ? 1.0F : exp2_of(rest > 0.0F ? __fmaf_rn(gap, k, gap * rest) : gap * k);
 	}
 
-	// sum of exp2((x - m)*k) over some pieces whose maximum is at most m; m = -infinity: of 0 (or NaN)
-	template <class T, int K>
-	__device__ __forceinline__ float sum_of_exp(const uint4 (&v)[K], float m, float k)
+	// Sum of exp2((x - m)*k) over some pieces whose maximum is at most m; m = -infinity: of 0 (or NaN). REST: k is rounded down and `rest`,
+	// above 0, is what that leaves out, which is then added to each argument: left out of every term it is a bias of the sum (1e-7 of it
+	// for scores a few tau apart), small against the rounding of one log probability, but not in a sequence's sum of them.
+	template <class T, int K, bool REST>
+	__device__ __forceinline__ float sum_of_exp(const uint4 (&v)[K], float m, float k, float rest)
 	{
 		constexpr int N = piece<T>::N;
 		const float base = m == -INFINITY ? 0.0F : m;
@@ -221,7 +224,7 @@ namespace nnf
 		{
 			// One fused operation for the argument, x*k - mk, where mk is m*k rounded: the sum is against 2^mk, and what mk is off by
 			// (2^-24 of it: 1e-6 for scores of 10, 0.04 at the limit) is put right on the sum.
-			const unsigned long long kk = pair_of(k, k), mm = pair_of(-mk, -mk);
+			const unsigned long long kk = pair_of(k, k), mm = pair_of(-mk, -mk), rr = pair_of(rest, rest);
 			unsigned long long both = pair_of(0.0F, 0.0F);
 			#pragma unroll
 			for (int j = 0; j < K; ++j)
@@ -232,12 +235,14 @@ namespace nnf
 				for (int e = 0; e < N; e += 2)
 				{
 					float a, b;
-					pair_apart(pair_fma(pair_of(f[e], f[e + 1]), kk, mm), a, b);
+					const unsigned long long x = pair_of(f[e], f[e + 1]);
+					pair_apart(REST ? pair_fma(x, rr, pair_fma(x, kk, mm)) : pair_fma(x, kk, mm), a, b);
 					both = pair_add(both, pair_of(exp2_of(a), exp2_of(b)));
 				}
 			}
 			pair_apart(both, s[0], s[1]);
-			return (s[0] + s[1]) * exp2_of(-__fmaf_rn(base, k, -mk));
+			const float off = __fmaf_rn(base, k, -mk);
+			return (s[0] + s[1]) * exp2_of(REST ? -__fmaf_rn(base, rest, off) : -off);
 		}
 		// larger ones (a row of nothing but the type's lowest value): the difference first
 		#pragma unroll
@@ -304,13 +309,17 @@ namespace nnf
 	}
 
 	// the elements of some pieces join a part
-	template <class T, int K>
-	__device__ __forceinline__ void add_part(softmax_part& part, const uint4 (&v)[K], float k)
+	template <class T, int K, bool REST = false>
+	__device__ __forceinline__ void add_part(softmax_part& part, const uint4 (&v)[K], float k, float rest = 0.0F)
 	{
 		const float m = fmaxf(part.m, piece<T>::template maximum<K>(v));
-		part.s = part.s * rescale(part.m, m, k) + sum_of_exp<T, K>(v, m, k);
+		part.s = part.s * rescale(part.m, m, k, REST ? rest : 0.0F) + sum_of_exp<T, K, REST>(v, m, k, rest);
 		part.m = m;
 	}
+
+	// ex2.approx.ftz is below 2^x by 2^-23 of it in the mean (its bound is 2^-22; for x = 0, as in the maximum's own term, it is exact): what
+	// a sum against its maximum is short of, for the reason given at sum_of_exp.
+	__device__ __forceinline__ float lifted(float s) { return s > 1.0F ? __fmaf_rn(s - 1.0F, 1.1920929e-7F, s) : s; }
 
 	__device__ __forceinline__ float vocab_warp_max(float v)
 	{

@@ -13,6 +13,8 @@
 // distributed shared memory. Maximum, sum and everything behind them are fp32; a gradient is rounded once, when it is stored.
 #include "nnf_vocab.cuh"
 
+#include <math.h>
+
 #include <type_traits>
 
 namespace nnf
@@ -34,6 +36,7 @@ namespace nnf
 			int cols;
 			int add;                   // the gradient is added to what dx holds
 			float tau, inv_tau, k;     // k = log2(e)/tau
+			float k_down, k_rest;      // the same, rounded down, and what that leaves out
 			int cluster;               // CTAs of a row
 			// targets
 			const void * tokens;
@@ -677,14 +680,14 @@ namespace nnf
 					const int at = i + (kScorePieces + j) * step + tid;
 					next[j] = at < hi ? __ldg(in + at) : nothing;
 				}
-				add_part<T, kScorePieces>(part, v, p.k);
+				add_part<T, kScorePieces, true>(part, v, p.k_down, p.k_rest);
 				#pragma unroll
 				for (int j = 0; j < kScorePieces; ++j)
 					v[j] = next[j];
 			}
 			{
 				const float m = vocab_warp_max(part.m);
-				part.s = vocab_warp_sum(part.s * rescale(part.m, m, p.k));
+				part.s = vocab_warp_sum(part.s * rescale(part.m, m, p.k_down, p.k_rest));
 				part.m = m;
 			}
 			if (split > 1)
@@ -709,8 +712,8 @@ namespace nnf
 					total.m = fmaxf(total.m, s_part[i].m);
 				total.m = vocab_warp_max(total.m);
 				for (int i = lane; i < (int)split * warps; i += 32)
-					total.s += s_part[i].s * rescale(s_part[i].m, total.m, p.k);
-				total.s = vocab_warp_sum(total.s);
+					total.s += s_part[i].s * rescale(s_part[i].m, total.m, p.k_down, p.k_rest);
+				total.s = lifted(vocab_warp_sum(total.s));
 				if (lane == 0)
 				{
 					const bool on = total.s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
@@ -801,7 +804,7 @@ namespace nnf
 					for (int j = 0; j < K; ++j)
 						v[j] = next[j];
 					fetch(i);
-					add_part<T, K>(part, v, p.k);
+					add_part<T, K, true>(part, v, p.k_down, p.k_rest);
 				}
 				#pragma unroll
 				for (int j = 0; j < K; ++j)
@@ -809,9 +812,9 @@ namespace nnf
 				const int64_t done = row;
 				const float its_xa = xa;
 				advance();
-				add_part<T, K>(part, v, p.k);
+				add_part<T, K, true>(part, v, p.k_down, p.k_rest);
 				const float m = vocab_warp_max(part.m);
-				const float s = vocab_warp_sum(part.s * rescale(part.m, m, p.k));
+				const float s = lifted(vocab_warp_sum(part.s * rescale(part.m, m, p.k_down, p.k_rest)));
 				if (lane == 0)
 				{
 					const bool on = s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
@@ -961,7 +964,7 @@ namespace nnf
 
 				softmax_part total;
 				total.m = vocab_warp_max(fmaxf(piece<T>::template maximum<NP>(v), at_edge));
-				total.s = vocab_warp_sum(sum_of_exp<T, NP>(v, total.m, p.k) + (at_edge == -INFINITY ? 0.0F : exp2_of((at_edge - total.m) * p.k)));
+				total.s = vocab_warp_sum(sum_of_exp<T, NP, false>(v, total.m, p.k, 0.0F) + (at_edge == -INFINITY ? 0.0F : exp2_of((at_edge - total.m) * p.k)));
 				bool on = total.s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
 				float c = 0.0F, at_token = 0.0F;
 				if (OP == kPolicy)
@@ -1490,6 +1493,9 @@ namespace nnf
 			p.tau = temperature;
 			p.inv_tau = 1.0F / temperature;
 			p.k = 1.44269502162933349609375F / temperature;
+			const double exact = 1.4426950408889634 / (double)temperature;
+			p.k_down = (float)exact > exact ? nextafterf((float)exact, 0.0F) : (float)exact;
+			p.k_rest = fmaxf((float)(exact - (double)p.k_down), 1.0e-37F);
 			switch (x.type)
 			{
 			case NNF_F32: return run_rows_of<float, OP>(s, p);
