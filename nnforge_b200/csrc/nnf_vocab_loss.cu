@@ -7,10 +7,15 @@
 //   every gradient is  dx_j = (what the targets hold at j) - c*p_j,  c one number for the row: the direction in which the loss falls,
 //   as the library's backward passes have it and its optimiser step adds it.
 //
-// All are bound by HBM: a row is read once, kept in registers while its maximum and sum are found (one exchange: a warp's maximum and
-// sum against it, joined by all warps), and its gradient written from there. A row that does not fit one CTA's registers, or that
-// would leave SMs idle because there are few rows, is split over a thread-block cluster, whose CTAs exchange their parts through
-// distributed shared memory. Maximum, sum and everything behind them are fp32; a gradient is rounded once, when it is stored.
+// HBM bounds them: an element is 2 or 4 bytes in (and as many out), and takes one or two exponentials. So a row is read once and stays
+// on chip between its sum and its gradient, in one of three places:
+//   short rows (up to 256 pieces of 16 bytes): a warp's registers, row after row (vocab_short_kernel)
+//   longer ones: the shared memory of a CTA, or of a thread-block cluster whose CTAs exchange maxima and sums (vocab_held_kernel)
+//   log probabilities alone need not be held (vocab_score_kernel, vocab_score_warp_kernel); their backward pass reads the row again
+//   (vocab_bwd_kernel), as does the loss of paired sequences, whose gradient needs the sums over all rows of a pair.
+// Rows of 16-bit scores are next to being bound by instructions too: per element an unpacking, a fused multiply-add, an exponential, a
+// sum and half a maximum, and for the gradient the first three again and half a rounding; fp32 arithmetic goes in pairs (f32x2). Maximum,
+// sum and everything behind them are fp32; a gradient is rounded once, when it is stored.
 #include "nnf_vocab.cuh"
 
 #include <math.h>
@@ -220,7 +225,18 @@ namespace nnf
 		// A CTA per row (a cluster, where the row is split), several of them on an SM. Bulk copies bring the row in, chunk by chunk; each
 		// chunk's exponentials are summed against the thread's running maximum as it arrives; the gradient is computed from shared memory.
 		// What an SM has in flight are the rows of its other CTAs: the bytes that a row takes up decide how many those are, so a
-		// quarter of a long row is held in registers.
+		// quarter of a long row is held in registers (four CTAs of 64 KB instead of three: 8192x32000 bf16 198 -> 178 us when it came; not for
+		// shorter rows, of which shared memory has room for more CTAs than registers do: 16384x12000 146 -> 154).
+		//
+		// One B200, policy loss, us (bytes at the copy rate of 6.55 TB/s): bf16 8192x32000 175 (160), 16384x12000 139 (120), 2048x131072 200 (164);
+		// fp32 8192x16000 159 (160), 1024x131072 183 (164). bf16 3000x32000 under the profiler: issue slots 59 %, exponentials (XU) 70 %, DRAM 54 %
+		// (writes still in L2 at the end not counted), 4 CTAs an SM. Twice the scores for the same bytes are why bf16 lies behind fp32; of a row
+		// that is split each CTA waits for the slowest of its cluster. Distillation of 64 kept logits takes 211 us for 8192x32000: the teacher's row,
+		// the loss and the kept columns lengthen a CTA's 10 us by 2.
+		//
+		// Measured and not kept: a persistent CTA an SM with the exponentials in registers and a ring of rows filled ahead of it (one row's
+		// chain of latencies at a time: 1.5 times the time), the gradient's exponentials by polynomial (issue slots are as short as the
+		// XU), warps of their own for the teacher's row (better for 16 kept logits, worse from 64 on).
 		constexpr int kHeldThreads = 256, kHeldChunk = 4, kHeldChunks = 40;   // kHeldChunk: pieces of a chunk that a thread takes
 
 		// kAnyRow: gradients that are added, or whose rows start elsewhere in their 16 bytes than the logits'; the loss alone.
@@ -614,6 +630,8 @@ namespace nnf
 
 		// ---- log probabilities alone: nothing to be held -----------------------------------------------------------------
 		// A CTA per row (a cluster, where there are few rows); a thread's next pieces are on their way while it sums the current ones.
+		// One B200, bf16, us (bytes at the copy rate): 8192x32000 88 (80), 2048x131072 87 (82), 64x32000 4 (a launch). XU 62 %, issue slots 57 %:
+		// what is left is the chain at either end of a row (token, first piece; sums, result).
 		constexpr int kScoreThreads = 256, kScorePieces = 4;
 
 		template <class T>
@@ -728,7 +746,8 @@ namespace nnf
 		}
 
 		// The same for many rows: a warp takes row after row, and a row's first pieces are asked for while the one before it ends. Lane l
-		// keeps the token of the l-th of the warp's next 32 rows, so that rows that count for nothing cost no time.
+		// keeps the token of the l-th of the warp's next 32 rows, so that rows that count for nothing cost no time. bf16, us (bytes at the
+		// copy rate; a CTA per row): 16384x12000 71 (60; 74), 32768x4096 52 (41; 83), 65536x1000 36 (20; 46).
 		constexpr int kRowWarps = 8;   // of a CTA
 
 		template <class T>
@@ -829,7 +848,9 @@ namespace nnf
 		}
 
 		// ---- short rows, with their gradient: a warp has a row in registers ---------------------------------------------------
-		// As above a warp takes row after row, and asks for the next one before it works on the one it has. NP: pieces of a lane.
+		// As above a warp takes row after row, and asks for the next one before it works on the one it has. NP: pieces of a lane. Policy loss,
+		// us (bytes at the copy rate; the row in a CTA's shared memory): bf16 65536x1000 67 (40; 147), 32768x2000 61 (40; 79), fp32 65536x1000
+		// 96 (80; 142). Bound by instructions: some 500 a row besides those of its scores.
 		template <class T, int OP, int NP, bool ANY>
 		__global__ void __launch_bounds__(kRowWarps * 32, NP > 4 ? 2 : 3) vocab_short_kernel(const vocab_params p)
 		{
@@ -1129,7 +1150,8 @@ namespace nnf
 		constexpr int kBwdThreads = 256, kBwdPieces = 4;
 
 		// ALIGNED: whole pieces are stored at once (the gradient is not added, and its rows start where the logits' do in their 16 bytes).
-		// The last row comes first: the end of the logits is what the forward pass before has left in L2.
+		// The last row comes first: the end of the logits is what the forward pass before has left in L2 (8192x32000 bf16, forward and backward,
+		// 265 -> 252 us). HBM bounds it: 8192x32000 with 30 % of the rows out moves 891 MB in 132 us, 6.8 TB/s with what comes from L2.
 		template <class T, bool ALIGNED>
 		__global__ void __launch_bounds__(kBwdThreads) vocab_bwd_kernel(const vocab_bwd_params p)
 		{
@@ -1219,7 +1241,9 @@ namespace nnf
 			return fmaxf(x, 0.0F) + log1pf(expf(-fabsf(x)));
 		}
 
-		// a CTA per pair; sums in double, in an order that depends on nothing but the lengths
+		// A CTA per pair; sums in double, in an order that depends on nothing but the lengths. 16 pairs of 8192 rows: 7 us, a chain of latencies
+		// (offsets, log probabilities, sums, loss, gradients) between two launches of 69 and 132 us. One launch for all three, in which resident CTAs
+		// drew the rows' items and a pair's gradients followed its sums while the scores were in L2, was measured at 217 us against 212 and dropped.
 		__global__ void __launch_bounds__(kPairThreads) vocab_pair_kernel(const pair_params p)
 		{
 			__shared__ double s_sum[2][kPairThreads / 32];
@@ -1397,7 +1421,8 @@ namespace nnf
 			int64_t cluster = 1;
 			while (cluster < kVocabCluster && pieces > cluster * 4200)
 				cluster *= 2;
-			// few rows: over more CTAs, as long as those are less than four an SM
+			// few rows: over more CTAs, as long as those are less than four an SM (32x32000 bf16 over 8 CTAs 5.4 us, over one 7.3; 148 rows over 2
+			// 7.2 us, over 4 8.6, over one 7.9)
 			while (cluster < kVocabCluster && v.rows * cluster * 2 < 4 * sm_count() && pieces > cluster * 512)
 				cluster *= 2;
 			if (tune().vocab_split > 0)
@@ -1407,7 +1432,7 @@ namespace nnf
 			p.v.cluster = (int)cluster;
 			p.error = device_error_word();
 			const int64_t per = div_up(pieces, cluster);
-			// 16 pieces a thread; where the SMs are not full, four
+			// 16 pieces a thread, so that little is spent on joining threads; where the SMs are not full, four (16x32000 5.4 us against 5.6..7.2)
 			int threads = (int)(div_up(div_up(per, v.rows * cluster < 4 * sm_count() ? 4 : 16), 32) * 32);
 			threads = threads < 64 ? 64 : threads > kHeldThreads ? kHeldThreads : threads;
 			const int64_t chunk = int64_t(threads) * kHeldChunk;
@@ -1431,8 +1456,10 @@ namespace nnf
 		int run_score(cudaStream_t s, vocab_params& p, int64_t pieces)
 		{
 			const int64_t slots = (int64_t)sm_count() * 4 * kRowWarps;
-			// warps: what the last turn of all of them leaves unused; CTAs: about 1.5 ns a row that starting and ending each costs
-			const int64_t idle = (div_up(p.rows, slots) * slots - p.rows) * pieces * 16 / 6500, turnover = p.rows * 3 / 2;
+			// In ns. Warps: what the last turn of all of them leaves unused; CTAs: 3/4 ns a row that starting and ending each costs. Warps / CTAs,
+			// us: 16384x12000 71 / 74, 8192x8192 29 / 32, 32768x4096 52 / 83; the other way round 8192x32000 103 / 88, 4096x16384 28.3 / 27.5,
+			// 1024x32000 22.7 / 15.8, 2048x131072 104 / 87
+			const int64_t idle = (div_up(p.rows, slots) * slots - p.rows) * pieces * 16 / 6500, turnover = p.rows * 3 / 4;
 			if (tune().vocab_form == 3 || (tune().vocab_form == 0 && idle < turnover))
 			{
 				const int64_t needed = div_up(p.rows, kRowWarps);
@@ -1478,6 +1505,7 @@ namespace nnf
 				return run_score<T>(s, p, pieces);
 			else
 			{
+				// a warp's registers hold 256 pieces (32768x2000 bf16 61 us, in shared memory 79); longer rows would spill them
 				if (pieces > 256 || tune().vocab_form == 2)
 					return run_held<T, OP>(s, p, pieces);
 				return pieces <= 32 ? run_short<T, OP, 1>(s, p) : pieces <= 64 ? run_short<T, OP, 2>(s, p) : pieces <= 128 ? run_short<T, OP, 4>(s, p) : run_short<T, OP, 8>(s, p);
