@@ -23,7 +23,6 @@ namespace nnf
 		{
 			return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
 		}
-		static __device__ __forceinline__ uint32_t bits(const float * p) { return __float_as_uint(*p); }
 		static __device__ __forceinline__ float value(const float * p) { return *p; }
 		static __device__ __forceinline__ void store(float * p, float v) { *p = v; }
 		static constexpr uint32_t kNothing = 0xff800000u;   // -infinity, in every element of the word
@@ -61,7 +60,6 @@ namespace nnf
 			}
 			return make_uint4(w[0], w[1], w[2], w[3]);
 		}
-		static __device__ __forceinline__ uint32_t bits(const __nv_bfloat16 * p) { return __bfloat16_as_ushort(*p); }
 		static __device__ __forceinline__ float value(const __nv_bfloat16 * p) { return __bfloat162float(*p); }
 		static __device__ __forceinline__ void store(__nv_bfloat16 * p, float v) { *p = __float2bfloat16_rn(v); }
 		static constexpr uint32_t kNothing = 0xff80ff80u;
@@ -102,7 +100,6 @@ namespace nnf
 			}
 			return make_uint4(w[0], w[1], w[2], w[3]);
 		}
-		static __device__ __forceinline__ uint32_t bits(const __half * p) { return __half_as_ushort(*p); }
 		static __device__ __forceinline__ float value(const __half * p) { return __half2float(*p); }
 		static __device__ __forceinline__ void store(__half * p, float v) { *p = __float2half_rn(v); }
 		static constexpr uint32_t kNothing = 0xfc00fc00u;
@@ -137,32 +134,6 @@ namespace nnf
 		__device__ __forceinline__ bool whole(int i) const { return (i > 0 || shift == 0) && (i + 1) * N - shift <= cols; }
 		__device__ __forceinline__ uint4 * address(int i) const { return reinterpret_cast<uint4 *>(at - shift) + i; }
 		__device__ __forceinline__ bool has(int i, int k) const { const int e = i * N - shift + k; return e >= 0 && e < cols; }
-
-		// elements outside the row: -infinity
-		__device__ __forceinline__ uint4 load(int i) const
-		{
-			if (whole(i))
-				return __ldcs(address(i));
-			uint32_t w[4];
-			#pragma unroll
-			for (int k = 0; k < 4; ++k)
-			{
-				w[k] = piece<T>::kNothing;
-				if (N == 4)
-				{
-					if (has(i, k))
-						w[k] = piece<T>::bits(at + i * N - shift + k);
-				}
-				else
-				{
-					if (has(i, 2 * k))
-						w[k] = (w[k] & 0xffff0000u) | piece<T>::bits(at + i * N - shift + 2 * k);
-					if (has(i, 2 * k + 1))
-						w[k] = (w[k] & 0xffffu) | (piece<T>::bits(at + i * N - shift + 2 * k + 1) << 16);
-				}
-			}
-			return make_uint4(w[0], w[1], w[2], w[3]);
-		}
 	};
 
 	// maximum and sum of exp2((x - maximum) * k) of some elements; nothing: (-infinity, 0)

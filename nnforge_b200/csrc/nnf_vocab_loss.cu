@@ -90,37 +90,19 @@ namespace nnf
 			end = within(end, p.rows);
 		}
 
-		// stores a piece of the gradient's row: whole and aligned pieces at once, others element by element
-		template <class T, class F>
-		__device__ __forceinline__ void store_piece(const row_frame<T>& x, T * dx, bool aligned, int i, int add, F f)
+		// a piece of a gradient that is nothing: at once where it is whole and starts at its 16 bytes, else element by element
+		template <class T>
+		__device__ __forceinline__ void clear_piece(const row_frame<T>& x, T * dx, bool aligned, int i)
 		{
-			constexpr int N = piece<T>::N;
-			const int first = i * N - x.shift;
+			const int first = i * piece<T>::N - x.shift;
 			if (aligned && x.whole(i))
-			{
-				uint4 * to = reinterpret_cast<uint4 *>(dx + first);
-				float g[N];
-				if (add)
-				{
-					piece<T>::unpack(*to, g);
-					#pragma unroll
-					for (int e = 0; e < N; ++e)
-						g[e] += f(e);
-				}
-				else
-				{
-					#pragma unroll
-					for (int e = 0; e < N; ++e)
-						g[e] = f(e);
-				}
-				__stcs(to, piece<T>::pack(g));
-			}
+				__stcs(reinterpret_cast<uint4 *>(dx + first), make_uint4(0, 0, 0, 0));
 			else
 			{
-				#pragma unroll
-				for (int e = 0; e < N; ++e)
+				#pragma unroll 1
+				for (int e = 0; e < piece<T>::N; ++e)
 					if (x.has(i, e))
-						piece<T>::store(dx + first + e, add ? piece<T>::value(dx + first + e) + f(e) : f(e));
+						piece<T>::store(dx + first + e, 0.0F);
 			}
 		}
 
@@ -168,8 +150,7 @@ namespace nnf
 		struct distill_shared
 		{
 			int * id;         // -1: the entry does not count
-			float * q;        // the teacher's probability
-			float * lnq;
+			float * q;        // the teacher's logit
 			float * x;        // the student's score
 			float * old;      // what the gradient held (it is added to)
 			uint32_t * seen;  // a bit for each of this CTA's columns
@@ -456,10 +437,13 @@ namespace nnf
 				part.s = vocab_warp_sum(part.s * rescale(part.m, m, p.k));
 				part.m = m;
 			}
-			// the first warp of every CTA gets every warp's part (and no CTA leaves before all have sent it theirs)
+			// The first warp of every CTA gets every warp's part (and no CTA leaves before all have sent it theirs). Where the gradient takes the
+			// scores' place, the other CTAs write over the token's score once they have this one's parts: it must be here by then.
 			if (split > 1)
 			{
 				vocab_cluster_wait();
+				if (OP == kPolicy && warp == 0 && lane == 0)
+					asm volatile("st.shared.f32 [%0], %1;" :: "r"(shared_address(&s_red[0][0])), "f"(xa) : "memory");   // (waits for it)
 				if (lane < (int)split)
 					vocab_cluster_send(s_part + rank * warps + warp, &s_exchanged, lane, part);
 				if (warp == 0)
@@ -887,7 +871,7 @@ namespace nnf
 				const row_frame<T> e(const_cast<T *>(static_cast<const T *>(p.x)) + r * p.ldx, p.cols);
 				T * const dx = static_cast<T *>(p.dx) + r * p.lddx;
 				for (int i = lane; i < e.pieces; i += 32)
-					store_piece<T>(e, dx, !ANY, i, 0, [](int) { return 0.0F; });
+					clear_piece<T>(e, dx, !ANY, i);
 			};
 			auto advance = [&]()
 			{
@@ -1178,7 +1162,7 @@ namespace nnf
 			{
 				if (!p.add)
 					for (int j = 0, i = from; j < kBwdPieces && i < x.pieces; ++j, i += step)
-						store_piece<T>(x, dx, ALIGNED, i, 0, [](int) { return 0.0F; });
+						clear_piece<T>(x, dx, ALIGNED, i);
 				return;
 			}
 			const row_gradient<T> gradient(m, p.k, -g / s);
@@ -1415,6 +1399,20 @@ namespace nnf
 			return check_launch("vocab_rows_kernel");
 		}
 
+		template <class K>
+		int allow_shared(K kernel, size_t bytes, const char * who)
+		{
+			constexpr size_t granted = 44 * 1024;   // of 48 KB without being asked for, static data among them
+			if (bytes <= granted)
+				return NNF_OK;
+			const int limit = running_config().max_shared_memory_per_block_optin - 4096;
+			if (bytes > (size_t)limit)
+				return set_error(NNF_ERR_UNSUPPORTED, "%s: %lld bytes of shared memory", who, (long long)bytes);
+			// the attribute is the kernel's: the same value whatever the shape, so that host threads do not lower it under each other's launches
+			const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
+			return e == cudaSuccess ? NNF_OK : set_error(NNF_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", who, cudaGetErrorString(e));
+		}
+
 		template <class T, int OP>
 		int run_held(cudaStream_t s, const vocab_params& v, int64_t pieces)
 		{
@@ -1442,13 +1440,9 @@ namespace nnf
 			p.slots = (int)((per - (registers ? chunk : 0) + 7) & ~int64_t(7));
 			const size_t smem = size_t(p.slots) * 16 + (OP == kDistill ? size_t(v.kept) * (aligned ? 12 : 16) + size_t(div_up(per * piece<T>::N, 32)) * 4 : 0);
 			auto kernel = registers ? vocab_held_kernel<T, OP, kRegisterRow> : aligned ? vocab_held_kernel<T, OP, kAlignedRow> : vocab_held_kernel<T, OP, kAnyRow>;
-			const int limit = running_config().max_shared_memory_per_block_optin - 4096;
-			if (smem > (size_t)limit)
-				return set_error(NNF_ERR_UNSUPPORTED, "vocab_held_kernel: %lld bytes", (long long)smem);
-			// the attribute is the kernel's: the same value whatever the shape, so that host threads do not lower it under each other's launches
-			const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
-			if (e != cudaSuccess)
-				return set_error(NNF_ERR_CUDA, "vocab_held_kernel: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+			const int st = allow_shared(kernel, smem, "vocab_held_kernel");
+			if (st != NNF_OK)
+				return st;
 			return launch_rows(kernel, v.rows * cluster, threads, smem, (int)cluster, s, p);
 		}
 
@@ -1487,10 +1481,9 @@ namespace nnf
 				(p.rows > 1 && (p.lddx - p.ldx) * (int64_t)sizeof(T) % 16 != 0);
 			auto kernel = any ? vocab_short_kernel<T, OP, NP, true> : vocab_short_kernel<T, OP, NP, false>;
 			const size_t smem = OP == kDistill ? size_t(kRowWarps) * 4 * (4 * size_t(p.kept) + NP * piece<T>::N + 1) : 0;
-			const int limit = running_config().max_shared_memory_per_block_optin - 4096;
-			const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
-			if (e != cudaSuccess)
-				return set_error(NNF_ERR_CUDA, "vocab_short_kernel: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+			const int st = allow_shared(kernel, smem, "vocab_short_kernel");
+			if (st != NNF_OK)
+				return st;
 			const int64_t needed = div_up(p.rows, kRowWarps), resident = (int64_t)sm_count() * (NP > 4 ? 2 : 3);
 			launch(kernel, needed < resident ? needed : resident, kRowWarps * 32, smem, s, p);
 			return check_launch("vocab_short_kernel");
