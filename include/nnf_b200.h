@@ -462,6 +462,8 @@ NNF_API int nnf_accuracy_fwd(nnf_stream_t stream, float * out, const float * pre
  * scores hold. Elsewhere infinities and NaN take their course.
  * As in every backward pass of this library, dlogits and dlogp are the direction in which the loss falls (its gradient negated: what
  * nnf_apply_gradient adds, and what nnf_softmax_nll_bwd adds to when both end in one buffer).
+ * No call needs a workspace. Kernels wait for nothing but their own copies and their own cluster; such a wait that runs out (5 s) raises
+ * the word of nnf_fused_error_check, value 4.
  * dlogits NULL: the loss alone. dlogits may be the logits themselves (same stride, not added to): each row's gradient takes its
  * scores' place (they overlap in no other way). add_to_destination accumulates into dlogits. The layers are losses: no output
  * errors, `scale` and the mask weigh them. */

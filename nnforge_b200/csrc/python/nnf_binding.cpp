@@ -267,7 +267,7 @@ namespace
 			const at::Tensor& t = THPVariable_Unpack(o);
 			if (!t.is_cuda() || t.layout() != at::kStrided)
 				fail(PyExc_AssertionError, name, "a CUDA tensor is expected");
-			else if (t.device().index() != c10::cuda::current_device())
+			else if (t.device().index() != current_device())
 				fail(PyExc_ValueError, name, "a tensor of the current device is expected");
 			return good ? &t : nullptr;
 		}
@@ -350,6 +350,13 @@ namespace
 		}
 
 	private:
+		int current_device()   // asked once a call
+		{
+			if (device < 0)
+				device = c10::cuda::current_device();
+			return device;
+		}
+
 		int type_of(const at::Tensor& t, const char * name, bool indices)
 		{
 			switch (t.scalar_type())
@@ -427,6 +434,7 @@ namespace
 		Py_ssize_t n, i = 0;
 		bool good = true;
 		nnf_stream_t given_stream = nullptr;
+		int device = -1;
 		std::vector<nnf_act> chain;
 	};
 
