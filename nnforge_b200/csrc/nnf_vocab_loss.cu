@@ -212,12 +212,13 @@ namespace nnf
 		// One B200, policy loss, us (bytes at the copy rate of 6.55 TB/s): bf16 8192x32000 175 (160), 16384x12000 139 (120), 2048x131072 200 (164);
 		// fp32 8192x16000 159 (160), 1024x131072 183 (164). bf16 3000x32000 under the profiler: issue slots 59 %, exponentials (XU) 70 %, DRAM 54 %
 		// (writes still in L2 at the end not counted), 4 CTAs an SM. Twice the scores for the same bytes are why bf16 lies behind fp32; of a row
-		// that is split each CTA waits for the slowest of its cluster. Distillation of 64 kept logits takes 211 us for 8192x32000: the teacher's row,
+		// that is split each CTA waits for the slowest of its cluster. Distillation of 64 kept logits takes 209 us for 8192x32000: the teacher's row,
 		// the loss and the kept columns lengthen a CTA's 10 us by 2.
 		//
 		// Measured and not kept: a persistent CTA an SM with the exponentials in registers and a ring of rows filled ahead of it (one row's
 		// chain of latencies at a time: 1.5 times the time), the gradient's exponentials by polynomial (issue slots are as short as the
-		// XU), warps of their own for the teacher's row (better for 16 kept logits, worse from 64 on).
+		// XU), warps of their own for the teacher's row (better for 16 kept logits, worse from 64 on), that row in front of
+		// the sums (its latency then keeps them from following the chunks: 4096x32000 with 64 kept logits 107 us against 104).
 		constexpr int kHeldThreads = 256, kHeldChunk = 4, kHeldChunks = 40;   // kHeldChunk: pieces of a chunk that a thread takes
 
 		// kAnyRow: gradients that are added, or whose rows start elsewhere in their 16 bytes than the logits'; the loss alone.
@@ -234,6 +235,7 @@ namespace nnf
 		struct held_result             // what the row comes to, found by the first warp
 		{
 			float m, s, c, at_token, share;
+			float t_max, t_sum;        // of the teacher's logits
 			int on;
 		};
 
@@ -246,7 +248,8 @@ namespace nnf
 			__shared__ uint64_t s_bar[kHeldChunks];
 			__shared__ uint64_t s_exchanged;
 			__shared__ held_result s_result;
-			__shared__ float s_red[2][kHeldThreads / 32];
+			__shared__ softmax_part s_teacher[kHeldThreads / 32];
+			__shared__ float s_score;
 			const vocab_params& p = hp.v;
 			const uint32_t split = (uint32_t)p.cluster;
 			const uint32_t rank = split > 1 ? vocab_cluster_rank() : 0;
@@ -280,6 +283,14 @@ namespace nnf
 			}
 			pdl_begin();
 
+			// a thread's first entry of the teacher's row: on its way before anything is waited for
+			int64_t id_first = -1;
+			float t_first = -INFINITY;
+			if (OP == kDistill && tid < p.kept)
+			{
+				id_first = index_at(p.ids, p.ids_wide, row * p.ld_ids + tid);
+				t_first = value_at(p.teacher, p.teacher_type, row * p.ld_teacher + tid);
+			}
 			const float w = p.mask ? __ldg(p.mask + row) : 1.0F;
 			int token = 0;
 			bool on = w != 0.0F;
@@ -357,7 +368,6 @@ namespace nnf
 			}
 			const float xa = OP == kPolicy && warp == 0 ? piece<T>::value(x.at + token) : 0.0F;
 			distill_shared d = {};
-			float t_max = 0.0F, t_sum = 0.0F;
 			// the score at a column of this CTA, in shared memory; elsewhere it was fetched with the teacher's row
 			auto place = [&](int id) { const int e = id + x.shift - from * N; return away && e >= 2 * chunk * N ? e - chunk * N : e; };
 			auto present = [&](int id)
@@ -372,42 +382,8 @@ namespace nnf
 				d.x = d.q + p.kept;
 				d.seen = reinterpret_cast<uint32_t *>(d.x + p.kept);
 				d.old = reinterpret_cast<float *>(d.seen + (per * N + 31) / 32);   // kAnyRow
-				// the teacher's row, while the student's is on its way
-				float m = -INFINITY;
-				for (int e = tid; e < p.kept; e += step)
-				{
-					const int64_t id = index_at(p.ids, p.ids_wide, row * p.ld_ids + e);
-					const bool in = id >= 0 && id < p.cols;
-					const float t = in ? value_at(p.teacher, p.teacher_type, row * p.ld_teacher + e) : -INFINITY;
-					const bool mine = in && id >= begin && id < begin + elements;
-					d.id[e] = in ? (int)id : -1;
-					d.q[e] = t;
-					if (in && (mine || rank == 0) && !present((int)id))
-						d.x[e] = piece<T>::value(x.at + id);   // (the first CTA finds the loss)
-					if (mine)
-						d.seen[((int)id - begin) >> 5] = 0;
-					if (ROW == kAnyRow && p.add && mine)
-						d.old[e] = piece<T>::value(dx + id);
-					m = fmaxf(m, t);
-				}
-				m = vocab_warp_max(m);
-				if (lane == 0)
-					s_red[0][warp] = m;
-				__syncthreads();
-				for (int i = 0; i < warps; ++i)
-					m = fmaxf(m, s_red[0][i]);
-				t_max = m == -INFINITY ? 0.0F : m;
-				float s = 0.0F;
-				for (int e = tid; e < p.kept; e += step)
-					s += exp2_of((d.q[e] - t_max) * p.k);
-				s = vocab_warp_sum(s);
-				if (lane == 0)
-					s_red[1][warp] = s;
 			}
 			__syncthreads();   // the barriers and the partial pieces are there
-			if (OP == kDistill)
-				for (int i = 0; i < warps; ++i)
-					t_sum += s_red[1][i];
 
 			// ---- maximum and sum, against the thread's running maximum ----
 			softmax_part part = {-INFINITY, 0.0F};
@@ -432,6 +408,32 @@ namespace nnf
 				for (int i = 0; i < chunks; ++i)
 					mbar_wait(s_bar + i, 0, again, hp.error);
 			}
+			if (OP == kDistill && warp * 32 < p.kept)
+			{
+				// the teacher's entries of this warp; its logits' maximum and sum are joined as the student's are
+				softmax_part teacher = {-INFINITY, 0.0F};
+				for (int e = tid; e < p.kept; e += step)
+				{
+					const int64_t id = e == tid ? id_first : index_at(p.ids, p.ids_wide, row * p.ld_ids + e);
+					const bool in = id >= 0 && id < p.cols, mine = in && id >= begin && id < begin + elements;
+					const float l = !in ? -INFINITY : e == tid ? t_first : value_at(p.teacher, p.teacher_type, row * p.ld_teacher + e);
+					d.id[e] = in ? (int)id : -1;
+					d.q[e] = l;
+					if (mine)
+						d.seen[((int)id - begin) >> 5] = 0;
+					if (ROW == kAnyRow && p.add && mine)
+						d.old[e] = piece<T>::value(dx + id);
+					if (in && (mine || rank == 0) && !present((int)id))   // (the first CTA finds the loss)
+						d.x[e] = piece<T>::value(x.at + id);
+					const float m = fmaxf(teacher.m, l);
+					teacher.s = teacher.s * rescale(teacher.m, m, p.k) + part_of(l).s * rescale(l, m, p.k);
+					teacher.m = m;
+				}
+				const float m = vocab_warp_max(teacher.m);
+				teacher.s = vocab_warp_sum(teacher.s * rescale(teacher.m, m, p.k));
+				if (lane == 0)
+					s_teacher[warp] = {m, teacher.s};
+			}
 			{
 				const float m = vocab_warp_max(part.m);
 				part.s = vocab_warp_sum(part.s * rescale(part.m, m, p.k));
@@ -443,11 +445,13 @@ namespace nnf
 			{
 				vocab_cluster_wait();
 				if (OP == kPolicy && warp == 0 && lane == 0)
-					asm volatile("st.shared.f32 [%0], %1;" :: "r"(shared_address(&s_red[0][0])), "f"(xa) : "memory");   // (waits for it)
+					asm volatile("st.shared.f32 [%0], %1;" :: "r"(shared_address(&s_score)), "f"(xa) : "memory");   // (waits for it)
 				if (lane < (int)split)
 					vocab_cluster_send(s_part + rank * warps + warp, &s_exchanged, lane, part);
 				if (warp == 0)
 					mbar_wait(&s_exchanged, 0, gave_up, hp.error);
+				if (OP == kDistill)
+					__syncthreads();   // the teacher's parts
 			}
 			else
 			{
@@ -465,7 +469,7 @@ namespace nnf
 					total.s += s_part[i].s * rescale(s_part[i].m, total.m, p.k);
 				total.s = vocab_warp_sum(total.s);
 				on = total.s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
-				held_result r = {total.m, total.s, 0.0F, 0.0F, 0.0F, on};
+				held_result r = {total.m, total.s, 0.0F, 0.0F, 0.0F, 0.0F, 0.0F, on};
 				if (OP == kPolicy)
 				{
 					const policy_row l = policy_of(p, xa, total, weight, __ldg(p.old_logp + row), __ldg(p.advantages + row), p.ref_logp ? __ldg(p.ref_logp + row) : 0.0F, on);
@@ -482,10 +486,13 @@ namespace nnf
 				}
 				else
 				{
-					on = on && t_sum != 0.0F && weight != 0.0F;
-					r.on = on;
-					r.c = on ? -weight * p.tau / total.s : 0.0F;
-					r.share = on ? weight * p.tau / t_sum : 0.0F;
+					const softmax_part mine = lane < min(warps, (p.kept + 31) / 32) ? s_teacher[lane] : softmax_part{-INFINITY, 0.0F};
+					const float top = vocab_warp_max(mine.m);
+					r.t_max = top == -INFINITY ? 0.0F : top;
+					r.t_sum = vocab_warp_sum(mine.s * rescale(mine.m, top, p.k));
+					r.on = on && r.t_sum != 0.0F && weight != 0.0F;
+					r.c = r.on ? -weight * p.tau / total.s : 0.0F;
+					r.share = r.on ? weight * p.tau / r.t_sum : 0.0F;
 				}
 				if (lane == 0)
 					s_result = r;
@@ -498,17 +505,17 @@ namespace nnf
 				float sum = 0.0F;
 				if (r.on)
 				{
-					const float ln = logf(r.s), t_ln = logf(t_sum);
+					const float ln = logf(r.s), t_ln = logf(r.t_sum);
 					for (int e = lane; e < p.kept; e += 32)
 					{
-						const float q = exp2_of((d.q[e] - t_max) * p.k);
+						const float q = exp2_of((d.q[e] - r.t_max) * p.k);
 						if (q != 0.0F)
 						{
 							const float xe = present(d.id[e]) ? piece<T>::value(held_at + place(d.id[e])) : d.x[e];
-							sum += q * (((d.q[e] - t_max) * p.inv_tau - t_ln) - ((xe - r.m) * p.inv_tau - ln));
+							sum += q * (((d.q[e] - r.t_max) * p.inv_tau - t_ln) - ((xe - r.m) * p.inv_tau - ln));
 						}
 					}
-					sum = vocab_warp_sum(sum) * (weight * p.tau * p.tau / t_sum);
+					sum = vocab_warp_sum(sum) * (weight * p.tau * p.tau / r.t_sum);
 				}
 				if (lane == 0)
 					p.loss[row] = sum;
@@ -590,7 +597,7 @@ namespace nnf
 					const int id = d.id[e];
 					if (id < begin || id >= begin + elements)
 						continue;
-					float q = exp2_of((d.q[e] - t_max) * p.k);
+					float q = exp2_of((d.q[e] - r.t_max) * p.k);
 					bool leads = true;
 					if (twice)
 					{
@@ -599,7 +606,7 @@ namespace nnf
 							if (d.id[o] == id)
 							{
 								leads = leads && o >= e;
-								q += exp2_of((d.q[o] - t_max) * p.k);
+								q += exp2_of((d.q[o] - r.t_max) * p.k);
 							}
 					}
 					if (leads)
