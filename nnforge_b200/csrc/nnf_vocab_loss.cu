@@ -1517,6 +1517,7 @@ namespace nnf
 		{
 			p.x = x.data; p.ldx = x.stride;
 			p.dx = dx ? dx->data : nullptr; p.lddx = dx ? dx->stride : 0;
+			p.add = dx && p.add;   // the loss alone is added to nothing: the kernels take `add` as leave to read what dx holds
 			p.rows = x.rows; p.cols = (int)x.cols;
 			p.tau = temperature;
 			p.inv_tau = 1.0F / temperature;
