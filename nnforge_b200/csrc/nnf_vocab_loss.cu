@@ -249,7 +249,7 @@ namespace nnf
 			__shared__ uint64_t s_exchanged;
 			__shared__ held_result s_result;
 			__shared__ softmax_part s_teacher[kHeldThreads / 32];
-			__shared__ float s_score;
+			__shared__ float s_number[2][32];
 			const vocab_params& p = hp.v;
 			const uint32_t split = (uint32_t)p.cluster;
 			const uint32_t rank = split > 1 ? vocab_cluster_rank() : 0;
@@ -291,7 +291,7 @@ namespace nnf
 				id_first = index_at(p.ids, p.ids_wide, row * p.ld_ids + tid);
 				t_first = value_at(p.teacher, p.teacher_type, row * p.ld_teacher + tid);
 			}
-			const float w = p.mask ? __ldg(p.mask + row) : 1.0F;
+			const float w = p.mask ? p.mask[row] : 1.0F;
 			int token = 0;
 			bool on = w != 0.0F;
 			if (OP == kPolicy)
@@ -366,7 +366,13 @@ namespace nnf
 				if (tid < N ? lo > 0 : hi < count)
 					held_at[(tid < N ? 0 : kept - 1) * N + e] = x.has(from + i, e) ? x.at[(from + i) * N - x.shift + e] : T(-INFINITY);
 			}
-			const float xa = OP == kPolicy && warp == 0 ? piece<T>::value(x.at + token) : 0.0F;
+			// what a policy's row comes to besides its sums, in the first warp: the token's score, and a number a lane (a load for all of them)
+			float xa = 0.0F, number = 0.0F;
+			if (OP == kPolicy && warp == 0)
+			{
+				xa = piece<T>::value(x.at + token);
+				number = (lane == 0 || (lane != 1 && !p.ref_logp) ? p.old_logp : lane == 1 ? p.advantages : p.ref_logp)[row];
+			}
 			distill_shared d = {};
 			// the score at a column of this CTA, in shared memory; elsewhere it was fetched with the teacher's row
 			auto place = [&](int id) { const int e = id + x.shift - from * N; return away && e >= 2 * chunk * N ? e - chunk * N : e; };
@@ -439,13 +445,18 @@ namespace nnf
 				part.s = vocab_warp_sum(part.s * rescale(part.m, m, p.k));
 				part.m = m;
 			}
-			// The first warp of every CTA gets every warp's part (and no CTA leaves before all have sent it theirs). Where the gradient takes the
-			// scores' place, the other CTAs write over the token's score once they have this one's parts: it must be here by then.
+			// The first warp of every CTA gets every warp's part (and no CTA leaves before all have sent it theirs). Once the other CTAs have this
+			// one's parts, they may write over what it still reads: the token's score, where the gradient takes the scores' place, and the
+			// row's numbers, where an output takes an input's (logp that of old_logp). They must be here by then.
 			if (split > 1)
 			{
 				vocab_cluster_wait();
-				if (OP == kPolicy && warp == 0 && lane == 0)
-					asm volatile("st.shared.f32 [%0], %1;" :: "r"(shared_address(&s_score)), "f"(xa) : "memory");   // (waits for it)
+				if (OP == kPolicy && warp == 0)
+				{
+					asm volatile("st.shared.f32 [%0], %1;" :: "r"(shared_address(s_number[0] + lane)), "f"(xa) : "memory");   // (waits for it)
+					asm volatile("st.shared.f32 [%0], %1;" :: "r"(shared_address(s_number[1] + lane)), "f"(number) : "memory");
+					__syncwarp();
+				}
 				if (lane < (int)split)
 					vocab_cluster_send(s_part + rank * warps + warp, &s_exchanged, lane, part);
 				if (warp == 0)
@@ -472,7 +483,9 @@ namespace nnf
 				held_result r = {total.m, total.s, 0.0F, 0.0F, 0.0F, 0.0F, 0.0F, on};
 				if (OP == kPolicy)
 				{
-					const policy_row l = policy_of(p, xa, total, weight, __ldg(p.old_logp + row), __ldg(p.advantages + row), p.ref_logp ? __ldg(p.ref_logp + row) : 0.0F, on);
+					auto of_lane = [&](int l) { return __shfl_sync(0xffffffffu, number, l); };
+					const float old_logp = of_lane(0), advantage = of_lane(1), ref_logp = of_lane(2);
+					const policy_row l = policy_of(p, xa, total, weight, old_logp, advantage, ref_logp, on);
 					r.c = l.c;
 					r.at_token = l.at_token;
 					r.on = l.c != 0.0F || l.at_token != 0.0F;
@@ -890,7 +903,7 @@ namespace nnf
 						return;
 					const int64_t r = base + lane * warps;
 					const bool there = r < p.rows;
-					const float w = !there ? 0.0F : p.mask ? __ldg(p.mask + r) : 1.0F;
+					const float w = !there ? 0.0F : p.mask ? p.mask[r] : 1.0F;
 					bool on = w != 0.0F;
 					weight = p.scale * w;
 					if (OP == kPolicy && there)
@@ -898,9 +911,9 @@ namespace nnf
 						const int64_t wide = index_at(p.tokens, p.tokens_wide, r);
 						on = on && wide >= 0 && wide < p.cols;
 						token = (int)wide;
-						old_logp = __ldg(p.old_logp + r);
-						advantage = __ldg(p.advantages + r);
-						ref_logp = p.ref_logp ? __ldg(p.ref_logp + r) : 0.0F;
+						old_logp = p.old_logp[r];
+						advantage = p.advantages[r];
+						ref_logp = p.ref_logp ? p.ref_logp[r] : 0.0F;
 					}
 					if (!on && there)
 					{
@@ -1244,6 +1257,8 @@ namespace nnf
 			int64_t begin[2], end[2];
 			double sum[2];
 			long long count[2];
+			// in front of the barrier: the rewards may take its place
+			const float ref[2] = {p.ref_logp[2 * pair], p.ref_logp[2 * pair + 1]};
 			#pragma unroll
 			for (int side = 0; side < 2; ++side)
 			{
@@ -1285,7 +1300,7 @@ namespace nnf
 				}
 				const double by = p.average && count[side] > 0 ? 1.0 / (double)count[side] : 1.0;
 				share[side] = (float)by;
-				gap[side] = sum[side] * by - (double)__ldg(p.ref_logp + 2 * pair + side);
+				gap[side] = sum[side] * by - (double)ref[side];
 				ratio[side] = (float)gap[side];
 			}
 			const double h = gap[0] - gap[1];

@@ -65,3 +65,65 @@ def test_the_loss_alone_is_added_to_nothing(capi, rows, cols, kept, dtype):
             given.append([torch.full(size, 7.0, device="cuda") for size in ((1,), (2,), (4,), (2, 4), (4,))])
             capi.preference_loss(*given[-1], x, tokens, offsets, torch.zeros(2, device="cuda"), add_to_destination=add)
         assert all(torch.equal(a, b) for a, b in zip(*given))
+
+
+# ---- outputs in the place of inputs that have an element for each row ----------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("split", [0, 2, 8])
+@pytest.mark.parametrize("rows,cols", [(3, 90), (200, 1500), (6, 5000), (12, 32000), (7, 70001), (300, 40000)])
+def test_outputs_in_the_place_of_inputs(capi, rows, cols, split, dtype):
+    """A row's numbers are read before another of its CTAs writes its results, so that both calls give the same bits; ratios are far from 1,
+    which is what a ratio of logp to itself would be."""
+    g = generator(rows * 3 + cols + split)
+    x = scores(g, rows, cols, TYPES[dtype])
+    tokens = torch.randint(0, cols, (rows,), device="cuda", generator=g)
+    tokens[rows // 2] = -100
+    old = (exact.token_logp(x, tokens, 1.0)[0] - 0.5 * torch.randn(rows, device="cuda", generator=g)).float()
+    adv, ref = torch.randn(rows, device="cuda", generator=g), old + 0.3 * torch.randn(rows, device="cuda", generator=g)
+    mask = (torch.rand(rows, device="cuda", generator=g) > 0.2).float() * 0.5
+    capi.set_tuning("vocab_split", split)
+
+    def policy(loss, logp, kl, old, adv, ref, mask):
+        dx = torch.full_like(x, 7.0)
+        capi.policy_loss(loss, logp, x, tokens, old, adv, ref_logp=ref, mask=mask, kl=kl, dlogits=dx, clip_low=0.2, clip_high=0.3, kl_coef=0.1)
+        return loss, logp, kl, dx
+
+    def copies():
+        return [v.clone() for v in (old, adv, ref, mask)]
+
+    want = policy(*(torch.empty(rows, device="cuda") for _ in range(3)), *copies())
+    for loss_at, logp_at, kl_at in ((1, 0, 2), (3, 2, 0), (0, 1, 3)):
+        given = copies()
+        got = policy(given[loss_at], given[logp_at], given[kl_at], *given)
+        for name, a, b in zip(("loss", "logp", "kl", "dlogits"), got, want):
+            assert torch.equal(a, b), (name, loss_at, logp_at, kl_at)
+    ids = torch.rand(rows, cols, device="cuda", generator=g).topk(20, dim=1).indices
+    top = torch.randn(rows, 20, device="cuda", generator=g)
+    results = []
+    for place in (False, True):
+        weights, dx = mask.clone(), torch.full_like(x, 7.0)
+        loss = weights if place else torch.empty(rows, device="cuda")
+        capi.distill_topk_loss(loss, x, ids, top, mask=weights, dlogits=dx)
+        results.append((loss, dx))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("average", [False, True])
+def test_rewards_in_the_place_of_the_reference(capi, average):
+    """Every thread of a pair's CTA takes the reference before one of them writes the rewards."""
+    g = generator(77)
+    x = scores(g, 3000, 40, torch.float32)
+    tokens = torch.randint(0, 40, (3000,), device="cuda", generator=g)
+    offsets = torch.arange(0, 3001, 3, device="cuda")
+    ref = torch.randn(1000, device="cuda", generator=g) * 4 - 9
+    results = []
+    for place in (False, True):
+        given = ref.clone()
+        rewards = given if place else torch.empty(1000, device="cuda")
+        loss, logp, saved, dlogp = torch.empty(500, device="cuda"), torch.empty(3000, device="cuda"), torch.empty(2, 3000, device="cuda"), torch.empty(3000, device="cuda")
+        dx = torch.empty_like(x)
+        capi.preference_loss(loss, rewards, logp, saved, dlogp, x, tokens, offsets, given, dlogits=dx, beta=0.5, average=average)
+        results.append((loss, rewards, logp, saved, dlogp, dx))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
