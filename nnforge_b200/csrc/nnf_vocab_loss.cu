@@ -1539,7 +1539,8 @@ namespace nnf
 			p.k = 1.44269502162933349609375F / temperature;
 			const double exact = 1.4426950408889634 / (double)temperature;
 			p.k_down = (float)exact > exact ? nextafterf((float)exact, 0.0F) : (float)exact;
-			p.k_rest = fmaxf((float)(exact - (double)p.k_down), 1.0e-37F);
+			// above 0, as it meets -infinity; no more above it than its type needs: beside a temperature of 1e37 k itself is 1e-37
+			p.k_rest = fmaxf((float)(exact - (double)p.k_down), 1.4e-45F);
 			switch (x.type)
 			{
 			case NNF_F32: return run_rows_of<float, OP>(s, p);

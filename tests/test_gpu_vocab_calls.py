@@ -127,3 +127,30 @@ def test_rewards_in_the_place_of_the_reference(capi, average):
         capi.preference_loss(loss, rewards, logp, saved, dlogp, x, tokens, offsets, given, dlogits=dx, beta=0.5, average=average)
         results.append((loss, rewards, logp, saved, dlogp, dx))
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+# ---- temperatures and sums ------------------------------------------------------------------------------------------
+
+
+@pytest.fixture(params=["built-in choice", "a CTA a row", "split", "warps"])
+def form(request, capi):
+    """The forms of the scoring kernels, whatever the sizes for which each is chosen."""
+    capi.set_tuning("vocab_form", {"b": 0, "a": 2, "s": 2, "w": 3}[request.param[0]])
+    capi.set_tuning("vocab_split", {"a": 1, "s": 4}.get(request.param[0], 0))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("tau", [1e30, 1e33, 1e37])
+@pytest.mark.parametrize("rows,cols", [(5, 700), (3, 20001)])
+def test_temperatures_as_large_as_the_scores(capi, form, rows, cols, tau, dtype):
+    """Scores of three times the temperature, as ordinary scores are at 1: no correction of the exponents may be larger than they are."""
+    g = generator(rows + cols)
+    x = scores(g, rows, cols, TYPES[dtype], spread=3.0 * tau)
+    x[0, cols // 2] = -float("inf")
+    tokens = torch.randint(0, cols, (rows,), device="cuda", generator=g)
+    tokens[0] = 0
+    logp, saved = torch.empty(rows, device="cuda"), torch.empty(2, rows, device="cuda")
+    capi.token_logp_fwd(logp, saved, x, tokens, temperature=tau)
+    want, want_saved, _, tol, _ = exact.token_logp(x, tokens, float(torch.tensor(tau, dtype=torch.float32)))
+    exact.check(logp, want, tol, "logp")
+    exact.check(saved[1], want_saved[1], 150 * exact.U * want_saved[1], "sum")
