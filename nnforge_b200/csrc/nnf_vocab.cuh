@@ -175,47 +175,55 @@ namespace nnf
 
 	// What a part's exponentials are multiplied with when the maximum becomes m. A part without a maximum (-infinity) keeps its sum: 0, or
 	// NaN where an element was NaN, which no maximum shows.
-	__device__ __forceinline__ float rescale(float part_m, float m, float k, float rest = 0.0F)
+	__device__ __forceinline__ float rescale(float part_m, float m, float k)
 	{
-		const float gap = part_m - m;
-		return part_m == m ? 1.0F : exp2_of(rest > 0.0F ? __fmaf_rn(gap, k, gap * rest) : gap * k);
+		return part_m == m ? 1.0F : exp2_of((part_m - m) * k);
 	}
 
-	// Sum of exp2((x - m)*k) over some pieces whose maximum is at most m; m = -infinity: of 0 (or NaN). REST: k is rounded down and `rest`,
-	// above 0, is what that leaves out, which is then added to each argument: left out of every term it is a bias of the sum (1e-7 of it
-	// for scores a few tau apart), small against the rounding of one log probability, but not in a sequence's sum of them.
+	// the same with what k leaves out (rest > 0)
+	__device__ __forceinline__ float rescale(float part_m, float m, float k, float rest)
+	{
+		const float gap = part_m - m;
+		return part_m == m ? 1.0F : exp2_of(__fmaf_rn(gap, k, gap * rest));
+	}
+
+	// From here on an argument leaves the fused form: x*k - mk is off by what mk was rounded by, 0.03 at this size.
+	constexpr float kFused = 1.0e6F;
+
+	// Sum of exp2(x*k - mk) over some pieces, with one fused operation for the argument. REST: k is rounded down and `rest`, above 0, is what
+	// that leaves out, which is then added to each argument: left out of every term it is a bias of the sum (1e-7 of it for scores a
+	// few tau apart), small against the rounding of one log probability, but not in a sequence's sum of them.
 	template <class T, int K, bool REST>
-	__device__ __forceinline__ float sum_of_exp(const uint4 (&v)[K], float m, float k, float rest)
+	__device__ __forceinline__ float sum_of_fused(const uint4 (&v)[K], float mk, float k, float rest)
 	{
 		constexpr int N = piece<T>::N;
-		const float base = m == -INFINITY ? 0.0F : m;
-		const float mk = base * k;
-		float s[2] = {0.0F, 0.0F};
-		if (fabsf(mk) < 1.0e6F)
+		const unsigned long long kk = pair_of(k, k), mm = pair_of(-mk, -mk), rr = pair_of(rest, rest);
+		unsigned long long both = pair_of(0.0F, 0.0F);
+		#pragma unroll
+		for (int j = 0; j < K; ++j)
 		{
-			// One fused operation for the argument, x*k - mk, where mk is m*k rounded: the sum is against 2^mk, and what mk is off by
-			// (2^-24 of it: 1e-6 for scores of 10, 0.04 at the limit) is put right on the sum.
-			const unsigned long long kk = pair_of(k, k), mm = pair_of(-mk, -mk), rr = pair_of(rest, rest);
-			unsigned long long both = pair_of(0.0F, 0.0F);
+			float f[N];
+			piece<T>::unpack(v[j], f);
 			#pragma unroll
-			for (int j = 0; j < K; ++j)
+			for (int e = 0; e < N; e += 2)
 			{
-				float f[N];
-				piece<T>::unpack(v[j], f);
-				#pragma unroll
-				for (int e = 0; e < N; e += 2)
-				{
-					float a, b;
-					const unsigned long long x = pair_of(f[e], f[e + 1]);
-					pair_apart(REST ? pair_fma(x, rr, pair_fma(x, kk, mm)) : pair_fma(x, kk, mm), a, b);
-					both = pair_add(both, pair_of(exp2_of(a), exp2_of(b)));
-				}
+				float a, b;
+				const unsigned long long x = pair_of(f[e], f[e + 1]);
+				pair_apart(REST ? pair_fma(x, rr, pair_fma(x, kk, mm)) : pair_fma(x, kk, mm), a, b);
+				both = pair_add(both, pair_of(exp2_of(a), exp2_of(b)));
 			}
-			pair_apart(both, s[0], s[1]);
-			const float off = __fmaf_rn(base, k, -mk);
-			return (s[0] + s[1]) * exp2_of(REST ? -__fmaf_rn(base, rest, off) : -off);
 		}
-		// larger ones (a row of nothing but the type's lowest value): the difference first
+		float s[2];
+		pair_apart(both, s[0], s[1]);
+		return s[0] + s[1];
+	}
+
+	// Sum of exp2((x - base)*k), the difference first: for scores beyond kFused (a row of nothing but the type's lowest value).
+	template <class T, int K>
+	__device__ __forceinline__ float sum_of_apart(const uint4 (&v)[K], float base, float k)
+	{
+		constexpr int N = piece<T>::N;
+		float s[2] = {0.0F, 0.0F};
 		#pragma unroll
 		for (int j = 0; j < K; ++j)
 		{
@@ -226,6 +234,21 @@ namespace nnf
 				s[e & 1] += exp2_of((f[e] - base) * k);
 		}
 		return s[0] + s[1];
+	}
+
+	// Sum of exp2((x - m)*k) over some pieces whose maximum is at most m; m = -infinity: of 0 (or NaN). rest: as above, 0 without.
+	template <class T, int K, bool REST = false>
+	__device__ __forceinline__ float sum_of_exp(const uint4 (&v)[K], float m, float k, float rest = 0.0F)
+	{
+		const float base = m == -INFINITY ? 0.0F : m;
+		const float mk = base * k;
+		if (fabsf(mk) < kFused)
+		{
+			// mk is m*k rounded: the fused sum is against 2^mk, and what mk is off by (2^-24 of it: 1e-6 for scores of 10) is put right on the sum
+			const float off = __fmaf_rn(base, k, -mk);
+			return sum_of_fused<T, K, REST>(v, mk, k, rest) * exp2_of(REST ? -__fmaf_rn(base, rest, off) : -off);
+		}
+		return sum_of_apart<T, K>(v, base, k);
 	}
 
 	// The gradient's c*exp2((x - m)*k) over a row. As in sum_of_exp the argument is one fused operation, and what m*k rounded is off by goes
@@ -243,7 +266,7 @@ namespace nnf
 			offset = sizeof(T) == 4 ? put_right : __log2f(fabsf(put_right)) - mk;
 			sign = c < 0.0F ? 0x80008000u : 0u;
 		}
-		__device__ __forceinline__ bool near() const { return fabsf(mk) < (sizeof(T) == 4 ? 1.0e6F : 256.0F); }
+		__device__ __forceinline__ bool near() const { return fabsf(mk) < (sizeof(T) == 4 ? kFused : 256.0F); }
 
 		template <bool NEAR> __device__ __forceinline__ uint4 whole(const uint4& v) const
 		{
@@ -280,17 +303,83 @@ namespace nnf
 	}
 
 	// the elements of some pieces join a part
-	template <class T, int K, bool REST = false>
-	__device__ __forceinline__ void add_part(softmax_part& part, const uint4 (&v)[K], float k, float rest = 0.0F)
+	template <class T, int K>
+	__device__ __forceinline__ void add_part(softmax_part& part, const uint4 (&v)[K], float k)
 	{
 		const float m = fmaxf(part.m, piece<T>::template maximum<K>(v));
-		part.s = part.s * rescale(part.m, m, k, REST ? rest : 0.0F) + sum_of_exp<T, K, REST>(v, m, k, rest);
+		part.s = part.s * rescale(part.m, m, k) + sum_of_exp<T, K>(v, m, k);
 		part.m = m;
 	}
 
-	// ex2.approx.ftz is below 2^x by 2^-23 of it in the mean (its bound is 2^-22; for x = 0, as in the maximum's own term, it is exact): what
-	// a sum against its maximum is short of, for the reason given at sum_of_exp.
-	__device__ __forceinline__ float lifted(float s) { return s > 1.0F ? __fmaf_rn(s - 1.0F, 1.1920929e-7F, s) : s; }
+	// The same over as many steps as a row has (512 where a warp takes a row of 1 MiB), no worse for their number: the sum carries what
+	// its roundings lose (confident rows, 1 and a hundred thousand small terms: off by up to 44*2^-24 without), and its reference moves only
+	// when the maximum is more than a factor of two above it, so that scores in ascending order do not multiply it with an approximate
+	// power at every step (20*2^-24 short, in the mean, over 131072). The reference stays an element: a row that is nearly one
+	// score has that score's own term exact.
+	struct running_part
+	{
+		float m;         // the maximum
+		float against;   // the reference, an element that is at most 1/k below the maximum; the sum is against it, or
+		float mk;        // against 2^mk where that is below kFused (against*k, rounded; 0 where there is no reference)
+		float s, lost;   // the sum, and what its roundings have added to it
+	};
+
+	__device__ __forceinline__ running_part running_none() { return {-INFINITY, -INFINITY, 0.0F, 0.0F, 0.0F}; }
+
+	// exponent of what the sum is against, less m*k (both with what k leaves out)
+	__device__ __forceinline__ float running_gap(const running_part& part, float m, float k, float rest)
+	{
+		if (fabsf(part.mk) < kFused)
+			return -__fmaf_rn(m, rest, __fmaf_rn(m, k, -part.mk));
+		const float gap = part.against - m;
+		return __fmaf_rn(gap, k, gap * rest);
+	}
+
+	// the part's sum against m, which is at least its maximum; without a reference it is 0, or NaN
+	__device__ __forceinline__ float running_sum(const running_part& part, float m, float k, float rest)
+	{
+		const float s = part.s - part.lost;
+		return part.against == -INFINITY ? s : s * exp2_of(running_gap(part, m, k, rest));
+	}
+
+	__device__ __forceinline__ void running_raise(running_part& part, float k, float rest)
+	{
+		const float mk = part.m * k;
+		if (part.against != -INFINITY)
+		{
+			float gap = running_gap(part, part.m, k, rest);
+			if (fabsf(mk) < kFused)
+				gap += __fmaf_rn(part.m, rest, __fmaf_rn(part.m, k, -mk));
+			const float share = exp2_of(gap);
+			part.s *= share;
+			part.lost *= share;
+		}
+		part.against = part.m;
+		part.mk = mk;
+	}
+
+	template <class T, int K>
+	__device__ __forceinline__ void add_running(running_part& part, const uint4 (&v)[K], float k, float rest)
+	{
+		part.m = fmaxf(part.m, piece<T>::template maximum<K>(v));
+		if ((part.m - part.against) * k > 1.0F)   // (both infinite: no)
+			running_raise(part, k, rest);
+		const float terms = fabsf(part.mk) < kFused ? sum_of_fused<T, K, true>(v, part.mk, k, rest) : sum_of_apart<T, K>(v, part.against, k);
+		const float more = terms - part.lost, s = part.s + more;
+		part.lost = (s - part.s) - more;
+		part.s = s;
+	}
+
+	// what a single element (none: -infinity) adds to a sum against m, which is at least it
+	__device__ __forceinline__ float edge_term(float x, float m, float k, float rest)
+	{
+		return x == -INFINITY ? 0.0F : (x - x + 1.0F) * rescale(x, m, k, rest);   // (infinity and NaN: NaN)
+	}
+
+	// ex2.approx.ftz is below 2^x by 0.83*2^-24 of it in the mean (measured over -20..0; 2.3*2^-24 at most; for x = 0, as in the maximum's own
+	// term, it is exact). A term has two of them, its own and its part's: what a sum against its maximum is short of, for the reason given
+	// at sum_of_fused.
+	__device__ __forceinline__ float lifted(float s) { return s > 1.0F ? __fmaf_rn(s - 1.0F, 9.9e-8F, s) : s; }
 
 	__device__ __forceinline__ float vocab_warp_max(float v)
 	{

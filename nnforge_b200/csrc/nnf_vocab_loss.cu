@@ -684,7 +684,8 @@ namespace nnf
 				v[j] = at < hi ? __ldg(in + at) : nothing;
 			}
 			float xa = 0.0F;
-			softmax_part part = {-INFINITY, 0.0F};
+			running_part own = running_none();
+			float at_edge = -INFINITY;
 			if (rank == 0 && tid == 0)
 				xa = piece<T>::value(x.at + token);
 			if (tid < 2 * N && from < to)
@@ -692,7 +693,7 @@ namespace nnf
 				// the partial pieces, an element a thread
 				const int at = tid < N ? from : to - 1, e = tid % N;
 				if ((tid < N ? lo > from : hi < to) && x.has(at, e))
-					part = part_of(piece<T>::value(x.at + at * N - x.shift + e));
+					at_edge = piece<T>::value(x.at + at * N - x.shift + e);
 			}
 			for (int i = lo; i < hi; i += kScorePieces * step)
 			{
@@ -702,16 +703,14 @@ namespace nnf
 					const int at = i + (kScorePieces + j) * step + tid;
 					next[j] = at < hi ? __ldg(in + at) : nothing;
 				}
-				add_part<T, kScorePieces, true>(part, v, p.k_down, p.k_rest);
+				add_running<T, kScorePieces>(own, v, p.k_down, p.k_rest);
 				#pragma unroll
 				for (int j = 0; j < kScorePieces; ++j)
 					v[j] = next[j];
 			}
-			{
-				const float m = vocab_warp_max(part.m);
-				part.s = vocab_warp_sum(part.s * rescale(part.m, m, p.k_down, p.k_rest));
-				part.m = m;
-			}
+			softmax_part part;
+			part.m = vocab_warp_max(fmaxf(own.m, at_edge));
+			part.s = vocab_warp_sum(running_sum(own, part.m, p.k_down, p.k_rest) + edge_term(at_edge, part.m, p.k_down, p.k_rest));
 			if (split > 1)
 			{
 				// the first CTA gets every warp's part
@@ -759,13 +758,13 @@ namespace nnf
 		{
 			constexpr int K = kScorePieces;
 			const int lane = (int)threadIdx.x & 31;
-			const int64_t warps = (int64_t)gridDim.x * kRowWarps;
+			const int warps = (int)gridDim.x * kRowWarps;   // of the launch: no more than are resident
 			const uint4 nothing = make_uint4(piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing, piece<T>::kNothing);
 			pdl_begin();
 			int64_t begin = 0, end = p.rows;
 			if (p.offsets)
 				covered_rows(p, begin, end);
-			int64_t base = begin + (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5) - 32 * warps;   // the first of 32 rows, `warps` apart
+			int64_t base = begin + (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5) - 32 * (int64_t)warps;   // the first of 32 rows, `warps` apart
 			uint32_t ahead = 0;          // those of them that count and are still to come
 			int token = 0;
 
@@ -775,13 +774,13 @@ namespace nnf
 			int lo = 0, hi = 0;
 			float xa = 0.0F, edge = -INFINITY;
 			uint4 next[K];
-			auto fetch = [&](int i)
+			auto fetch = [&](int i, auto first)
 			{
 				#pragma unroll
 				for (int j = 0; j < K; ++j)
 				{
 					const int at = i + j * 32 + lane;
-					next[j] = at >= lo && at < hi ? __ldg(x.address(at)) : nothing;
+					next[j] = (!first.value || at >= lo) && at < hi ? __ldg(x.address(at)) : nothing;
 				}
 			};
 			auto advance = [&]()
@@ -792,7 +791,7 @@ namespace nnf
 					base += 32 * warps;
 					if (base >= end)
 						return;
-					const int64_t r = base + lane * warps;
+					const int64_t r = base + (int64_t)lane * warps;
 					const int64_t wide = r < end ? index_at(p.tokens, p.tokens_wide, r) : -1;
 					const bool on = wide >= 0 && wide < p.cols;
 					token = (int)wide;
@@ -806,38 +805,42 @@ namespace nnf
 				}
 				const int l = __ffs((int)ahead) - 1;
 				ahead &= ahead - 1;
-				row = base + l * warps;
+				row = base + (int64_t)l * warps;
 				x = row_frame<T>(const_cast<T *>(static_cast<const T *>(p.x)) + row * p.ldx, p.cols);
 				lo = x.whole(0) ? 0 : 1;
 				hi = x.whole(x.pieces - 1) ? x.pieces : x.pieces - 1;
-				fetch(0);
+				fetch(0, std::true_type());
 				xa = piece<T>::value(x.at + __shfl_sync(0xffffffffu, token, l));
 				if (lo > 0 || hi < x.pieces)
 					edge = edge_of(x, lane);
 			};
 			for (advance(); row >= 0;)
 			{
-				softmax_part part = {-INFINITY, 0.0F};
-				if (lo > 0 || hi < x.pieces)
-					part = part_of(edge);
+				running_part part = running_none();
+				const bool steps = hi > K * 32, ragged = lo > 0 || hi < x.pieces;
 				uint4 v[K];
 				for (int i = K * 32; i < hi; i += K * 32)
 				{
 					#pragma unroll
 					for (int j = 0; j < K; ++j)
 						v[j] = next[j];
-					fetch(i);
-					add_part<T, K, true>(part, v, p.k_down, p.k_rest);
+					fetch(i, std::false_type());
+					add_running<T, K>(part, v, p.k_down, p.k_rest);
 				}
 				#pragma unroll
 				for (int j = 0; j < K; ++j)
 					v[j] = next[j];
 				const int64_t done = row;
-				const float its_xa = xa;
+				const float its_xa = xa, at_edge = ragged ? edge : -INFINITY;
 				advance();
-				add_part<T, K, true>(part, v, p.k_down, p.k_rest);
-				const float m = vocab_warp_max(part.m);
-				const float s = lifted(vocab_warp_sum(part.s * rescale(part.m, m, p.k_down, p.k_rest)));
+				// the last step, and the only one of a short row: against the row's maximum at once
+				const float m = vocab_warp_max(fmaxf(fmaxf(part.m, at_edge), piece<T>::template maximum<K>(v)));
+				float sum = sum_of_exp<T, K, true>(v, m, p.k_down, p.k_rest);
+				if (ragged)
+					sum += edge_term(at_edge, m, p.k_down, p.k_rest);
+				if (steps)
+					sum += running_sum(part, m, p.k_down, p.k_rest);
+				const float s = lifted(vocab_warp_sum(sum));
 				if (lane == 0)
 				{
 					const bool on = s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
@@ -989,7 +992,7 @@ namespace nnf
 
 				softmax_part total;
 				total.m = vocab_warp_max(fmaxf(piece<T>::template maximum<NP>(v), at_edge));
-				total.s = vocab_warp_sum(sum_of_exp<T, NP, false>(v, total.m, p.k, 0.0F) + (at_edge == -INFINITY ? 0.0F : exp2_of((at_edge - total.m) * p.k)));
+				total.s = vocab_warp_sum(sum_of_exp<T, NP>(v, total.m, p.k) + (at_edge == -INFINITY ? 0.0F : exp2_of((at_edge - total.m) * p.k)));
 				bool on = total.s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
 				float c = 0.0F, at_token = 0.0F;
 				if (OP == kPolicy)
