@@ -42,6 +42,7 @@ namespace nnf
 			int add;                   // the gradient is added to what dx holds
 			float tau, inv_tau, k;     // k = log2(e)/tau
 			float k_down, k_rest;      // the same, rounded down, and what that leaves out
+			float inv_rest;            // 1/tau less inv_tau
 			int cluster;               // CTAs of a row
 			// targets
 			const void * tokens;
@@ -104,6 +105,17 @@ namespace nnf
 					if (x.has(i, e))
 						piece<T>::store(dx + first + e, 0.0F);
 			}
+		}
+
+		// (xa - M)/tau - ln S, rounded once: what a reciprocal that is rounded to 32 bits loses has one sign in every row (1.4*2^-24 in the mean
+		// at a temperature of 1.7), which a sequence's sum gathers
+		__device__ __forceinline__ float logp_of(const vocab_params& p, float xa, float m, float s)
+		{
+			const float gap = xa - m, ln = -logf(s), h = gap * p.inv_tau;
+			const float lost = __fmaf_rn(gap, p.inv_rest, __fmaf_rn(gap, p.inv_tau, -h));   // of h
+			const float sum = __fadd_rn(h, ln), back = sum - h;
+			const float less = (h - (sum - back)) + (ln - back);                           // of the sum
+			return h == -INFINITY ? h + ln : sum + (lost + less);
 		}
 
 		// what a policy's row comes to
@@ -738,7 +750,7 @@ namespace nnf
 				if (lane == 0)
 				{
 					const bool on = total.s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
-					p.logp[row] = on ? (xa - total.m) * p.inv_tau - logf(total.s) : 0.0F;
+					p.logp[row] = on ? logp_of(p, xa, total.m, total.s) : 0.0F;
 					if (p.saved)
 					{
 						p.saved[row] = on ? total.m : 0.0F;
@@ -844,7 +856,7 @@ namespace nnf
 				if (lane == 0)
 				{
 					const bool on = s != 0.0F;   // NaN counts; a row of nothing but -infinity does not
-					p.logp[done] = on ? (its_xa - m) * p.inv_tau - logf(s) : 0.0F;
+					p.logp[done] = on ? logp_of(p, its_xa, m, s) : 0.0F;
 					if (p.saved)
 					{
 						p.saved[done] = on ? m : 0.0F;
@@ -1539,6 +1551,7 @@ namespace nnf
 			p.rows = x.rows; p.cols = (int)x.cols;
 			p.tau = temperature;
 			p.inv_tau = 1.0F / temperature;
+			p.inv_rest = (float)(1.0 / (double)temperature - (double)p.inv_tau);
 			p.k = 1.44269502162933349609375F / temperature;
 			const double exact = 1.4426950408889634 / (double)temperature;
 			p.k_down = (float)exact > exact ? nextafterf((float)exact, 0.0F) : (float)exact;

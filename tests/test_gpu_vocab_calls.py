@@ -189,3 +189,23 @@ def test_long_sums(capi, form, rows, what, dtype, cols):
     error = error_of_sums(x, saved, 1.0)
     assert float(error.abs().max()) <= 120.0
     assert abs(float(error.mean())) <= 4.0
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("tau", [0.7, 1.0, 1.5, 1.7])
+def test_the_mean_error_of_log_probabilities(capi, form, tau, dtype):
+    """What a sequence's sum gathers. Roundings to nearest have no sign; what has one is k = log2(e)/tau and 1/tau as floats (2u and 0.5u of
+    them at these temperatures, u = 2^-24, times scores that are several tau apart) and the approximate powers, 0.83u short each: two a
+    term are put back, a term has one to three. So 0.83u, four standard errors of 8192 rows that are off by 5u each (0.22u), and 0.2u for
+    the logarithm."""
+    rows, cols = 8192, 16000
+    g = generator(16)
+    x = torch.randn(rows, cols, device="cuda", generator=g) * 2.5
+    tokens = torch.randint(0, cols, (rows,), device="cuda", generator=g)
+    x.scatter_add_(1, tokens[:, None], 4.0 + 4.0 * torch.rand(rows, 1, device="cuda", generator=g))
+    x = x.to(TYPES[dtype])
+    logp = torch.empty(rows, device="cuda")
+    capi.token_logp_fwd(logp, None, x, tokens, temperature=tau)
+    tau = float(torch.tensor(tau, dtype=torch.float32))
+    error = torch.cat([logp[r:r + 1024].double() - exact.token_logp(x[r:r + 1024], tokens[r:r + 1024], tau)[0] for r in range(0, rows, 1024)]) / exact.U
+    assert abs(float(error.mean())) <= 1.25
