@@ -463,7 +463,7 @@ NNF_API int nnf_accuracy_fwd(nnf_stream_t stream, float * out, const float * pre
  * As in every backward pass of this library, dlogits and dlogp are the direction in which the loss falls (its gradient negated: what
  * nnf_apply_gradient adds, and what nnf_softmax_nll_bwd adds to when both end in one buffer).
  * No call needs a workspace. Kernels wait for nothing but their own copies and their own cluster; such a wait that runs out (5 s) raises
- * the word of nnf_fused_error_check, value 4.
+ * the word of nnf_fused_error_check, value 4, and the row's results are NaN.
  * dlogits NULL: the loss alone. dlogits may be the logits themselves (same stride, not added to): each row's gradient takes its
  * scores' place (they overlap in no other way). What is read with one element for each row or sequence may be given as an output of the
  * same call too (logp in old_logp's place, kl in ref_logp's, loss in the mask's, rewards in ref_logp's): it is read before it is written.

@@ -187,8 +187,10 @@ namespace nnf
 				: "=r"(done) : "r"(shared_address(b)), "r"(phase), "r"(1000000u) : "memory");   // suspended for up to a millisecond
 			return done != 0;
 		}
-		// Bounded: when the limit runs out the error word is raised and the caller carries on, without waiting any more; every loop has
-		// its number of turns from the start, so that all threads still meet at the same barriers and leave.
+		// Bounded: when the limit runs out the error word is raised and the caller carries on, without waiting any more for what this flag
+		// stands for; every loop has its number of turns from the start, so that all threads still meet at the same barriers and leave. The
+		// row's sum is then made NaN, which its results show, and what has not come is waited for once more, since it would be written
+		// into the shared memory of a CTA that has left. Nothing covers what takes longer than both waits.
 		__device__ __forceinline__ void mbar_wait(uint64_t * b, uint32_t phase, bool& gave_up, int * error)
 		{
 			if (gave_up || mbar_try(b, phase))
@@ -422,9 +424,10 @@ namespace nnf
 				add_part<T, kHeldChunk>(part, own, p.k);
 			if (gave_up)
 			{
-				bool again = false;   // nobody leaves while a copy may still write into this CTA's shared memory
+				bool again = false;
 				for (int i = 0; i < chunks; ++i)
 					mbar_wait(s_bar + i, 0, again, hp.error);
+				part.s = NAN;
 			}
 			if (OP == kDistill && warp * 32 < p.kept)
 			{
@@ -457,9 +460,10 @@ namespace nnf
 				part.s = vocab_warp_sum(part.s * rescale(part.m, m, p.k));
 				part.m = m;
 			}
-			// The first warp of every CTA gets every warp's part (and no CTA leaves before all have sent it theirs). Once the other CTAs have this
+			// The first warp of every CTA gets every warp's part (and the CTA leaves only then). Once the other CTAs have this
 			// one's parts, they may write over what it still reads: the token's score, where the gradient takes the scores' place, and the
 			// row's numbers, where an output takes an input's (logp that of old_logp). They must be here by then.
+			bool late = false;   // another CTA's parts
 			if (split > 1)
 			{
 				vocab_cluster_wait();
@@ -472,7 +476,15 @@ namespace nnf
 				if (lane < (int)split)
 					vocab_cluster_send(s_part + rank * warps + warp, &s_exchanged, lane, part);
 				if (warp == 0)
-					mbar_wait(&s_exchanged, 0, gave_up, hp.error);
+				{
+					mbar_wait(&s_exchanged, 0, late, hp.error);
+					if (late)
+					{
+						bool again = false;
+						mbar_wait(&s_exchanged, 0, again, hp.error);
+					}
+					__syncwarp();
+				}
 				if (OP == kDistill)
 					__syncthreads();   // the teacher's parts
 			}
@@ -484,7 +496,7 @@ namespace nnf
 			}
 			if (warp == 0)
 			{
-				softmax_part total = {-INFINITY, 0.0F};
+				softmax_part total = {-INFINITY, late ? NAN : 0.0F};
 				for (int i = lane; i < (int)split * warps; i += 32)
 					total.m = fmaxf(total.m, s_part[i].m);
 				total.m = vocab_warp_max(total.m);
