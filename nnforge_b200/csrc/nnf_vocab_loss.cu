@@ -140,8 +140,11 @@ namespace nnf
 			{
 				const float gap = ref_logp - r.logp, grown = expm1f(gap);
 				r.kl = grown - gap;
-				loss += p.kl_coef * r.kl;
-				g += p.kl_coef * grown;
+				if (p.kl_coef != 0.0F)   // (0 * infinity is no number)
+				{
+					loss += p.kl_coef * r.kl;
+					g += p.kl_coef * grown;
+				}
 			}
 			g = weight != 0.0F ? g * weight * p.inv_tau : 0.0F;
 			r.loss = weight != 0.0F ? loss * weight : 0.0F;

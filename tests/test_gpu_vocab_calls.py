@@ -209,3 +209,25 @@ def test_the_mean_error_of_log_probabilities(capi, form, tau, dtype):
     tau = float(torch.tensor(tau, dtype=torch.float32))
     error = torch.cat([logp[r:r + 1024].double() - exact.token_logp(x[r:r + 1024], tokens[r:r + 1024], tau)[0] for r in range(0, rows, 1024)]) / exact.U
     assert abs(float(error.mean())) <= 1.25
+
+
+# ---- terms whose coefficient is 0 ------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,cols", [(6, 100), (5, 5000), (3, 70001)])
+def test_a_divergence_that_is_only_watched(capi, rows, cols):
+    """kl_coef 0: the reference changes neither loss nor gradient, also where the divergence is infinite (a score of -infinity; logp < -100)."""
+    g = generator(cols)
+    x = scores(g, rows, cols, torch.float32)
+    tokens = torch.randint(0, cols, (rows,), device="cuda", generator=g)
+    x[0, tokens[0]] = -float("inf")
+    x[1, tokens[1]] = -200.0
+    old, adv, ref = torch.full((rows,), -3.0, device="cuda"), torch.randn(rows, device="cuda", generator=g), torch.full((rows,), -2.0, device="cuda")
+    results = []
+    for r in (None, ref):
+        loss, logp, kl, dx = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda"), torch.full_like(x, 7.0)
+        capi.policy_loss(loss, logp, x, tokens, old, adv, ref_logp=r, kl=kl, dlogits=dx)
+        results.append((loss, logp, dx))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    assert bool(torch.isfinite(results[1][0]).all()) and bool(torch.isfinite(results[1][2]).all())
+    assert float(kl[1]) == float("inf") and bool(torch.isfinite(kl[2:]).all())
