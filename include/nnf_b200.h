@@ -459,7 +459,7 @@ NNF_API int nnf_accuracy_fwd(nnf_stream_t stream, float * out, const float * pre
  *
  * A row counts for nothing where its token is outside [0, cols), its mask (a weight for each row, may be NULL: 1) is 0, or all its
  * scores are -infinity. Such a row is not read (but in the last case): its loss, logp and kl are 0, its gradient is 0, whatever its
- * scores hold. Elsewhere infinities and NaN take their course; a term of a loss whose coefficient (kl_coef)
+ * scores hold. Elsewhere infinities and NaN take their course; a term of a loss whose coefficient (kl_coef, label_smoothing and 1 less it)
  * is 0 is left out, whatever its value.
  * As in every backward pass of this library, dlogits and dlogp are the direction in which the loss falls (its gradient negated: what
  * nnf_apply_gradient adds, and what nnf_softmax_nll_bwd adds to when both end in one buffer).

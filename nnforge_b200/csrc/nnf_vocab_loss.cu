@@ -1344,7 +1344,7 @@ namespace nnf
 			else
 			{
 				const float m = (float)(h * (double)p.beta);
-				loss = (1.0F - p.smoothing) * softplus(-m) + p.smoothing * softplus(m);
+				loss = (p.smoothing < 1.0F ? (1.0F - p.smoothing) * softplus(-m) : 0.0F) + (p.smoothing > 0.0F ? p.smoothing * softplus(m) : 0.0F);
 				dh = p.beta * (p.smoothing / (1.0F + expf(-m)) - (1.0F - p.smoothing) / (1.0F + expf(m)));
 			}
 			if (threadIdx.x == 0)

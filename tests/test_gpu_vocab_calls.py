@@ -231,3 +231,20 @@ def test_a_divergence_that_is_only_watched(capi, rows, cols):
     assert all(torch.equal(a, b) for a, b in zip(*results))
     assert bool(torch.isfinite(results[1][0]).all()) and bool(torch.isfinite(results[1][2]).all())
     assert float(kl[1]) == float("inf") and bool(torch.isfinite(kl[2:]).all())
+
+
+@pytest.mark.parametrize("smoothing", [0.0, 1.0])
+def test_a_sequence_that_is_impossible(capi, smoothing):
+    """The sequence that is to lose has a token of probability 0: no loss and no gradient without the other term of label smoothing."""
+    g = generator(5)
+    x = scores(g, 8, 50, torch.float32)
+    tokens = torch.randint(0, 50, (8,), device="cuda", generator=g)
+    loser = 5 if smoothing == 0.0 else 1   # of the first sequence, rows 0..3, or the second
+    x[loser, tokens[loser]] = -float("inf")
+    loss, rewards = torch.empty(1, device="cuda"), torch.empty(2, device="cuda")
+    logp, dlogp, saved = torch.empty(8, device="cuda"), torch.empty(8, device="cuda"), torch.empty(2, 8, device="cuda")
+    dx = torch.full_like(x, 7.0)
+    capi.preference_loss(loss, rewards, logp, saved, dlogp, x, tokens, torch.tensor([0, 4, 8], device="cuda"), torch.zeros(2, device="cuda"), dlogits=dx, beta=0.5,
+                         label_smoothing=smoothing)
+    assert float(loss[0]) == 0.0 and not bool(dlogp.any()) and not bool(dx.any())
+    assert float(rewards[1 if smoothing == 0.0 else 0]) == -float("inf")
