@@ -466,7 +466,7 @@ NNF_API int nnf_accuracy_fwd(nnf_stream_t stream, float * out, const float * pre
  * No call needs a workspace. Kernels wait for nothing but their own copies and their own cluster; such a wait that runs out (5 s) raises
  * the word of nnf_fused_error_check, value 4, and the row's results are NaN.
  * dlogits NULL: the loss alone. dlogits may be the logits themselves (same stride, not added to): each row's gradient takes its
- * scores' place (they overlap in no other way). What is read with one element for each row or sequence may be given as an output of the
+ * scores' place (any other overlap is refused). What is read with one element for each row or sequence may be given as an output of the
  * same call too (logp in old_logp's place, kl in ref_logp's, loss in the mask's, rewards in ref_logp's): it is read before it is written.
  * add_to_destination accumulates into dlogits. The layers are losses: no output
  * errors, `scale` and the mask weigh them. */

@@ -1406,6 +1406,29 @@ namespace nnf
 			return NNF_OK;
 		}
 
+		// whether an element of one matrix lies in the other (of the same type and shape); what lies between rows belongs to neither
+		bool overlap(const nnf_matrix& a, const nnf_matrix& b)
+		{
+			const int64_t size = element_size(a.type), width = a.cols * size;
+			const int64_t step_a = (a.rows > 1 ? a.stride : a.cols) * size, step_b = (b.rows > 1 ? b.stride : b.cols) * size;
+			const int64_t apart = (int64_t)(reinterpret_cast<uintptr_t>(b.data) - reinterpret_cast<uintptr_t>(a.data));
+			if (apart >= (a.rows - 1) * step_a + width || -apart >= (b.rows - 1) * step_b + width)
+				return false;
+			if (step_a == step_b)
+			{
+				const int64_t within = (apart % step_a + step_a) % step_a;   // of b's rows, in the steps of a
+				return within < width || within > step_a - width;
+			}
+			for (int64_t r = 0; r < a.rows; ++r)   // rows side by side in one buffer, with strides of their own
+			{
+				const int64_t reach = r * step_a - apart;   // from b's first row to this one
+				int64_t next = reach < width ? 0 : (reach - width) / step_b + 1;   // the first row of b that ends behind this one's start
+				if (next < b.rows && next * step_b < reach + width)
+					return true;
+			}
+			return false;
+		}
+
 		// logits, and their gradient if there is one
 		int check_logits(const char * who, const nnf_matrix * x, const nnf_matrix * dx, int add, float temperature)
 		{
@@ -1426,6 +1449,8 @@ namespace nnf
 					return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: dlogits have another type or shape than the logits", who);
 				if (dx->data == x->data && x->rows > 0 && (add || dx->stride != x->stride))
 					return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: dlogits in the logits' place: with their stride, and not added to", who);
+				if (dx->data != x->data && x->rows > 0 && overlap(*x, *dx))
+					return set_error(NNF_ERR_INVALID_ARGUMENT, "%s: dlogits overlap the logits", who);
 			}
 			return NNF_OK;
 		}

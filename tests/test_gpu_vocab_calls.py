@@ -248,3 +248,32 @@ def test_a_sequence_that_is_impossible(capi, smoothing):
                          label_smoothing=smoothing)
     assert float(loss[0]) == 0.0 and not bool(dlogp.any()) and not bool(dx.any())
     assert float(rewards[1 if smoothing == 0.0 else 0]) == -float("inf")
+
+
+# ---- where the gradient lies -----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 40), (6, 100), (5, 5001), (3, 40000)])
+@pytest.mark.parametrize("layout", ["side by side", "every second row", "strides of their own", "one behind the other"])
+def test_gradients_in_the_logits_buffer(capi, rows, cols, layout):
+    """Logits and gradient in one buffer without a shared element, their rows between each other's: not refused, and right."""
+    g = generator(rows + cols)
+    buffer = torch.full((8 * rows * cols + 64,), 7.0, device="cuda")
+    if layout == "side by side":
+        x, dx = (torch.as_strided(buffer, (rows, cols), (3 * cols, 1), at) for at in (0, 2 * cols))
+    elif layout == "every second row":
+        x, dx = (torch.as_strided(buffer, (rows, cols), (2 * cols, 1), at) for at in (cols, 0))
+    elif layout == "strides of their own":
+        x, dx = torch.as_strided(buffer, (rows, cols), (2 * cols, 1), 0), torch.as_strided(buffer, (rows, cols), (4 * cols, 1), cols)
+    else:
+        x, dx = torch.as_strided(buffer, (rows, cols), (cols, 1), rows * cols), torch.as_strided(buffer, (rows, cols), (cols, 1), 0)
+    x.copy_(scores(g, rows, cols, torch.float32))
+    was = x.clone()
+    tokens = torch.randint(0, cols, (rows,), device="cuda", generator=g)
+    logp, saved, up = torch.empty(rows, device="cuda"), torch.empty(2, rows, device="cuda"), torch.randn(rows, device="cuda", generator=g)
+    capi.token_logp_fwd(logp, saved, x, tokens)
+    capi.token_logp_bwd(dx, up, x, tokens, saved)
+    _, _, on, _, p = exact.token_logp(was, tokens, 1.0)
+    want, size = exact.gradient(p, tokens, on, up.double(), up.double().abs(), 1.0)
+    exact.check(dx, want, exact.GRAD * size, "dlogits")
+    assert torch.equal(x, was) and int((buffer == 7.0).sum()) == buffer.numel() - 2 * rows * cols
