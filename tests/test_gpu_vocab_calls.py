@@ -277,3 +277,97 @@ def test_gradients_in_the_logits_buffer(capi, rows, cols, layout):
     want, size = exact.gradient(p, tokens, on, up.double(), up.double().abs(), 1.0)
     exact.check(dx, want, exact.GRAD * size, "dlogits")
     assert torch.equal(x, was) and int((buffer == 7.0).sum()) == buffer.numel() - 2 * rows * cols
+
+
+# ---- corners ---------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("kept", [341, 700, 1024])
+@pytest.mark.parametrize("cols", [30, 1000])
+def test_many_kept_logits_of_short_rows(capi, cols, kept, dtype):
+    """More shared memory than a launch has without asking for it; more entries than columns, so that most are there several times."""
+    g = generator(cols + kept)
+    x = scores(g, 50, cols, TYPES[dtype])
+    ids = torch.randint(-2, cols + 2, (50, kept), device="cuda", generator=g)
+    ids[7] = -1
+    top = torch.randn(50, kept, device="cuda", generator=g)
+    mask = torch.rand(50, device="cuda", generator=g)
+    for add in (False, True):
+        loss, dx = torch.empty(50, device="cuda"), torch.zeros_like(x)
+        capi.distill_topk_loss(loss, x, ids, top, mask=mask, dlogits=dx, add_to_destination=add)
+        want = exact.distill(x, ids, top, mask, 1.0, 1.0)
+        exact.check(loss, *want["loss"], "loss")
+        exact.check(dx, *want["dlogits"], "dlogits")
+
+
+def test_pairs_without_rows(capi):
+    """Two pairs and no row at all: the reference alone decides."""
+    x, none, tokens = torch.empty(0, 100, device="cuda"), torch.empty(0, device="cuda"), torch.empty(0, dtype=torch.int64, device="cuda")
+    ref = torch.tensor([1.0, 3.0, -2.0, -5.0], device="cuda")
+    for squared in (False, True):
+        loss, rewards = torch.full((2,), 7.0, device="cuda"), torch.full((4,), 7.0, device="cuda")
+        capi.preference_loss(loss, rewards, none, torch.empty(2, 0, device="cuda"), none, x, tokens, torch.zeros(5, dtype=torch.int64, device="cuda"), ref,
+                             dlogits=torch.empty_like(x), kind=capi.PREFERENCE_SQUARED if squared else capi.PREFERENCE_LOGISTIC, beta=0.5)
+        h = torch.tensor([2.0, -3.0], dtype=torch.float64)   # q = -ref
+        want = (h - 1.0) ** 2 if squared else torch.nn.functional.softplus(-0.5 * h)
+        # beta*h is exact; the logistic loss has an exponential, a logarithm and a sum of a few roundings each
+        exact.check(loss, want, 16 * exact.U * (want + 1.0), "loss")
+        assert rewards.tolist() == [-0.5, -1.5, 1.0, 2.5]
+
+
+@pytest.mark.parametrize("cols", [5000, 131072])
+def test_references_on_either_side_of_the_fused_arguments(capi, form, cols):
+    """Scores of about 7e5, where x*k passes the 1e6 from which the difference is taken first, in ascending and in descending order, and rows that
+    begin with the type's lowest value: parts of both kinds are joined. Scores are multiples of 2^-4, |x - M| < 30."""
+    g = generator(cols)
+    border = 1.0e6 / 1.4426950408889634
+    line = (torch.linspace(-15.0, 15.0, cols, device="cuda", dtype=torch.float64) * 16).round() / 16
+    rows = torch.stack([sign * (round(border) + line) for sign in (1.0, -1.0)] + [sign * (round(border) - line) for sign in (1.0, -1.0)]).float()
+    low = torch.randn(3, cols, device="cuda", generator=g)
+    low[0, :cols // 2] = torch.finfo(torch.float32).min
+    low[1, cols // 2:] = torch.finfo(torch.float32).min
+    low[2, 1::2] = -1.0e6
+    x = torch.cat([rows, low])
+    tokens = x.argmax(dim=1)
+    tokens[1::2] = (tokens[1::2] + 7) % cols
+    logp, saved = torch.empty(7, device="cuda"), torch.empty(2, 7, device="cuda")
+    capi.token_logp_fwd(logp, saved, x, tokens)
+    want, want_saved, _, tol, _ = exact.token_logp(x, tokens, 1.0)
+    exact.check(logp, want, tol, "logp")
+    exact.check(saved[0], want_saved[0], torch.zeros_like(tol), "maximum")
+    exact.check(saved[1], want_saved[1], 150 * exact.U * want_saved[1], "sum")
+
+
+def test_a_step_of_training_returns_its_losses(capi):
+    """Policy loss and distillation into one gradient: both losses, and the gradient, against their definitions."""
+    g = generator(22)
+    rows, cols = 96, 1500
+    x = scores(g, rows, cols, torch.float32)
+    tokens = torch.randint(0, cols, (rows,), device="cuda", generator=g)
+    tokens[5] = -100
+    logp64 = exact.token_logp(x, tokens, 1.0)[0]
+    moved = 0.1 * torch.randn(rows, device="cuda", generator=g).double().clamp(-1.5, 1.5)   # ratios within the borders
+    old, adv, ref = (logp64 - moved).float(), torch.randn(rows, device="cuda", generator=g), (logp64 + 0.3).float()
+    ids = torch.rand(rows, cols, device="cuda", generator=g).topk(12, dim=1).indices
+    top = torch.randn(rows, 12, device="cuda", generator=g)
+    loss, logp, dloss, dx = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda"), torch.empty_like(x)
+    capi.policy_loss(loss, logp, x, tokens, old, adv, ref_logp=ref, kl_coef=0.1, dlogits=dx, scale=1.0 / rows)
+    capi.distill_topk_loss(dloss, x, ids, top, dlogits=dx, scale=0.5 / rows, add_to_destination=True)
+    policy, teacher = exact.policy(x, tokens, old, adv, ref, None, 0.2, 0.2, 0.1, 1.0, 1.0 / rows), exact.distill(x, ids, top, None, 1.0, 0.5 / rows)
+    exact.check(loss, *policy["loss"], "policy loss")
+    exact.check(dloss, *teacher["loss"], "distillation")
+    a, b = policy["dlogits"], teacher["dlogits"]
+    exact.check(dx, a[0] + b[0], a[1] + b[1] + 2 * exact.U * (a[0].abs() + b[0].abs()), "dlogits")
+
+
+def test_offsets_that_are_wrong_touch_nothing_in_front(capi):
+    """Offsets below 0, behind the last row or decreasing: the memory on either side of every output stays as it was."""
+    x = scores(generator(12), 12, 100, torch.float32)
+    tokens = torch.randint(0, 100, (12,), device="cuda", generator=generator(13))
+    for offsets in ([-5, 4, 40], [8, 4, 2], [0, 50, 12], [20, 30, 40], [-9, -7, -3]):
+        guard = torch.full((5, 64), 7.0, device="cuda")
+        loss, rewards, logp, dlogp, saved = guard[0, 16:17], guard[1, 16:18], guard[2, 16:28], guard[3, 16:28], guard[4, 16:40].view(2, 12)
+        capi.preference_loss(loss, rewards, logp, saved, dlogp, x, tokens, torch.tensor(offsets, device="cuda"), torch.zeros(2, device="cuda"))
+        for row, count in zip(guard, (1, 2, 12, 12, 24)):
+            assert bool((row[:16] == 7.0).all()) and bool((row[16 + count:] == 7.0).all())
