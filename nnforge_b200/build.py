@@ -5,7 +5,8 @@
 -fmad=false for every file whose kernels are held to nnForge's plain (CPU) backend bit for bit: there products
 and sums must be rounded separately. The single-launch training batch norm (nnf_bn_chain.cu, nnf_bn_cluster.cu) is a tolerance
 row - the reference's arithmetic there is cuDNN's - and is built with contraction: its launches are bound by
-how instruction issue and memory overlap, and every fused multiply-add is an instruction less.
+how instruction issue and memory overlap, and every fused multiply-add is an instruction less. So are the losses on the scores of a
+vocabulary (nnf_vocab_loss.cu), which the reference does not have.
 """
 import os
 import subprocess

@@ -226,10 +226,10 @@ namespace nnf
 		// quarter of a long row is held in registers (four CTAs of 64 KB instead of three: 8192x32000 bf16 198 -> 178 us when it came; not for
 		// shorter rows, of which shared memory has room for more CTAs than registers do: 16384x12000 146 -> 154).
 		//
-		// One B200, policy loss, us (bytes at the copy rate of 6.55 TB/s): bf16 8192x32000 175 (160), 16384x12000 139 (120), 2048x131072 200 (164);
-		// fp32 8192x16000 159 (160), 1024x131072 183 (164). bf16 3000x32000 under the profiler: issue slots 59 %, exponentials (XU) 70 %, DRAM 54 %
+		// One B200, policy loss, us (bytes at the copy rate of 6.55 TB/s): bf16 8192x32000 172 (160), 16384x12000 136 (120), 2048x131072 195 (164);
+		// fp32 8192x16000 157 (160), 1024x131072 181 (164). bf16 3000x32000 under the profiler: issue slots 60 %, exponentials (XU) 70 %, DRAM 54 %
 		// (writes still in L2 at the end not counted), 4 CTAs an SM. Twice the scores for the same bytes are why bf16 lies behind fp32; of a row
-		// that is split each CTA waits for the slowest of its cluster. Distillation of 64 kept logits takes 209 us for 8192x32000: the teacher's row,
+		// that is split each CTA waits for the slowest of its cluster. Distillation of 64 kept logits takes 208 us for 8192x32000: the teacher's row,
 		// the loss and the kept columns lengthen a CTA's 10 us by 2.
 		//
 		// Measured and not kept: a persistent CTA an SM with the exponentials in registers and a ring of rows filled ahead of it (one row's
@@ -661,7 +661,7 @@ namespace nnf
 
 		// ---- log probabilities alone: nothing to be held -----------------------------------------------------------------
 		// A CTA per row (a cluster, where there are few rows); a thread's next pieces are on their way while it sums the current ones.
-		// One B200, bf16, us (bytes at the copy rate): 8192x32000 88 (80), 2048x131072 87 (82), 64x32000 4 (a launch). XU 62 %, issue slots 57 %:
+		// One B200, bf16, us (bytes at the copy rate): 8192x32000 87 (80), 2048x131072 86 (82), 64x32000 4.5 (a launch). XU 72 %, issue slots 68 %, DRAM 69 %:
 		// what is left is the chain at either end of a row (token, first piece; sums, result).
 		constexpr int kScoreThreads = 256, kScorePieces = 4;
 
@@ -777,7 +777,8 @@ namespace nnf
 
 		// The same for many rows: a warp takes row after row, and a row's first pieces are asked for while the one before it ends. Lane l
 		// keeps the token of the l-th of the warp's next 32 rows, so that rows that count for nothing cost no time. bf16, us (bytes at the
-		// copy rate; a CTA per row): 16384x12000 71 (60; 74), 32768x4096 52 (41; 83), 65536x1000 36 (20; 46).
+		// copy rate; a CTA per row): 16384x12000 70 (60; 75), 32768x4096 52 (41; 85), 65536x1000 36 (20; 47; issue slots 66 %, XU 47 %, DRAM 41 %:
+		// what a row costs besides its scores, and its latencies).
 		constexpr int kRowWarps = 8;   // of a CTA
 
 		template <class T>
@@ -883,8 +884,9 @@ namespace nnf
 
 		// ---- short rows, with their gradient: a warp has a row in registers ---------------------------------------------------
 		// As above a warp takes row after row, and asks for the next one before it works on the one it has. NP: pieces of a lane. Policy loss,
-		// us (bytes at the copy rate; the row in a CTA's shared memory): bf16 65536x1000 67 (40; 147), 32768x2000 61 (40; 79), fp32 65536x1000
-		// 96 (80; 142). Bound by instructions: some 500 a row besides those of its scores.
+		// us (bytes at the copy rate; the row in a CTA's shared memory): bf16 65536x1000 68 (40; 150), 32768x2000 61 (40; 80), fp32 65536x1000
+		// 96 (80; 140). Bound by latencies: at 65536x1000 issue slots are busy 63 %, XU 56 %, DRAM 36 %; in 80 registers five warps a scheduler are
+		// resident, each of which has an instruction ready every 8 cycles, so that a third of the cycles have none. A row takes 700.
 		template <class T, int OP, int NP, bool ANY>
 		__global__ void __launch_bounds__(kRowWarps * 32, NP > 4 ? 2 : 3) vocab_short_kernel(const vocab_params p)
 		{
@@ -1185,7 +1187,7 @@ namespace nnf
 
 		// ALIGNED: whole pieces are stored at once (the gradient is not added, and its rows start where the logits' do in their 16 bytes).
 		// The last row comes first: the end of the logits is what the forward pass before has left in L2 (8192x32000 bf16, forward and backward,
-		// 265 -> 252 us). HBM bounds it: 8192x32000 with 30 % of the rows out moves 891 MB in 132 us, 6.8 TB/s with what comes from L2.
+		// 265 -> 252 us when it came). HBM bounds it: 8192x32000 with 30 % of the rows out moves 891 MB in 132 us, 6.8 TB/s with what comes from L2.
 		template <class T, bool ALIGNED>
 		__global__ void __launch_bounds__(kBwdThreads) vocab_bwd_kernel(const vocab_bwd_params p)
 		{
@@ -1496,8 +1498,8 @@ namespace nnf
 			int64_t cluster = 1;
 			while (cluster < kVocabCluster && pieces > cluster * 4200)
 				cluster *= 2;
-			// few rows: over more CTAs, as long as those are less than four an SM (32x32000 bf16 over 8 CTAs 5.4 us, over one 7.3; 148 rows over 2
-			// 7.2 us, over 4 8.6, over one 7.9)
+			// few rows: over more CTAs, as long as those are less than four an SM (32x32000 bf16 over 8 CTAs 4.8 us, over one 7.1; 148 rows over 2
+			// 7.1 us, over 4 8.5, over one 7.5)
 			while (cluster < kVocabCluster && v.rows * cluster * 2 < 4 * sm_count() && pieces > cluster * 512)
 				cluster *= 2;
 			if (tune().vocab_split > 0)
@@ -1507,7 +1509,8 @@ namespace nnf
 			p.v.cluster = (int)cluster;
 			p.error = device_error_word();
 			const int64_t per = div_up(pieces, cluster);
-			// 16 pieces a thread, so that little is spent on joining threads; where the SMs are not full, four (16x32000 5.4 us against 5.6..7.2)
+			// 16 pieces a thread, so that little is spent on joining threads; where the SMs are not full, four (16x32000 5.0 us, with eight
+			// or 16 5.5; 256x32000 9.5, with 16 9.8)
 			int threads = (int)(div_up(div_up(per, v.rows * cluster < 4 * sm_count() ? 4 : 16), 32) * 32);
 			threads = threads < 64 ? 64 : threads > kHeldThreads ? kHeldThreads : threads;
 			const int64_t chunk = int64_t(threads) * kHeldChunk;
@@ -1528,8 +1531,8 @@ namespace nnf
 		{
 			const int64_t slots = (int64_t)sm_count() * 4 * kRowWarps;
 			// In ns. Warps: what the last turn of all of them leaves unused; CTAs: 3/4 ns a row that starting and ending each costs. Warps / CTAs,
-			// us: 16384x12000 71 / 74, 8192x8192 29 / 32, 32768x4096 52 / 83; the other way round 8192x32000 103 / 88, 4096x16384 28.3 / 27.5,
-			// 1024x32000 22.7 / 15.8, 2048x131072 104 / 87
+			// us: 16384x12000 70 / 75, 8192x8192 29 / 32, 32768x4096 52 / 85; the other way round 8192x32000 102 / 87, 4096x16384 28.1 / 27.6,
+			// 1024x32000 22.7 / 15.3, 2048x131072 102 / 86
 			const int64_t idle = (div_up(p.rows, slots) * slots - p.rows) * pieces * 16 / 6500, turnover = p.rows * 3 / 4;
 			if (tune().vocab_form == 3 || (tune().vocab_form == 0 && idle < turnover))
 			{
@@ -1544,8 +1547,8 @@ namespace nnf
 				cluster = tune().vocab_split < kVocabCluster ? tune().vocab_split : kVocabCluster;
 			p.cluster = (int)cluster;
 			int threads = (int)(div_up(div_up(div_up(pieces, cluster), 8), 32) * 32);
-			// 128 threads a row: twice the rows of 256 are in flight, so that fewer of them are at their start or end (8192x32000 bf16 85.8
-			// against 90.7 us, 3000x50000 53.5 / 56.5); 256 where that leaves the last turn emptier (2048x131072 86 against 90 us, 300x65536 10.9 / 11.7)
+			// 128 threads a row: twice the rows of 256 are in flight, so that fewer of them are at their start or end (8192x32000 bf16 87
+			// against 94 us, 3000x50000 54 / 58); 256 where that leaves the last turn emptier (2048x131072 86 against 89 us, 300x65536 12.7 / 14.5)
 			const int most = p.rows < 4 * sm_count() || (pieces > 8192 && p.rows < 16 * sm_count()) ? kScoreThreads : kScoreThreads / 2;
 			threads = threads > most ? most : threads;
 			return launch_rows(vocab_score_kernel<T>, p.rows * cluster, threads, 0, (int)cluster, s, p);
@@ -1575,7 +1578,7 @@ namespace nnf
 				return run_score<T>(s, p, pieces);
 			else
 			{
-				// a warp's registers hold 256 pieces (32768x2000 bf16 61 us, in shared memory 79); longer rows would spill them
+				// a warp's registers hold 256 pieces (32768x2000 bf16 61 us, in shared memory 80); longer rows would spill them
 				if (pieces > 256 || tune().vocab_form == 2)
 					return run_held<T, OP>(s, p, pieces);
 				return pieces <= 32 ? run_short<T, OP, 1>(s, p) : pieces <= 64 ? run_short<T, OP, 2>(s, p) : pieces <= 128 ? run_short<T, OP, 4>(s, p) : run_short<T, OP, 8>(s, p);
