@@ -428,8 +428,8 @@ def softmax_nll_bwd(dlogits, probs, targets, mask=None, scale=1.0, add_to_destin
 # Losses on the scores of a vocabulary. Logits [rows][vocabulary] are fp32, bf16 or fp16, contiguous within a row (rows may be further
 # apart); tokens, teacher_ids and offsets are int32 or int64; everything else is fp32 with one element for each row, unless stated.
 # A row whose token lies outside the vocabulary (-100, say), whose mask is 0 or whose scores are all -infinity counts for nothing:
-# loss, log probability and gradient are 0. dlogits may be the logits themselves; as everywhere in the library it is the direction in which
-# the loss falls, what apply_gradient adds.
+# loss, log probability and gradient are 0. dlogits may be the logits themselves (no other overlap), and an output with an element for each row
+# an input that has one; as everywhere in the library dlogits is the direction in which the loss falls, what apply_gradient adds.
 
 
 def token_logp_fwd(logp, saved, logits, tokens, temperature=1.0, stream=None):

@@ -936,7 +936,8 @@ namespace
 		float * loss = a.floats(o_loss, "loss", pairs), * rewards = a.floats(o_rewards, "rewards", 2 * pairs), * logp = a.floats(o_logp, "logp", x.rows);
 		float * saved = a.floats(o_saved, "saved", 2 * x.rows), * dlogp = a.floats(o_dlogp, "dlogp", x.rows);
 		const float * ref_logp = a.floats(a.next(), "ref_logp", 2 * pairs);
-		const int kind = (int)a.integer();
+		const long long asked = a.integer();
+		const int kind = asked == (int)asked ? (int)asked : -1;   // no kind either
 		const float beta = (float)a.number(), smoothing = (float)a.number();
 		const int average = a.flag();
 		const float tau = (float)a.number(), scale = (float)a.number();

@@ -371,3 +371,12 @@ def test_offsets_that_are_wrong_touch_nothing_in_front(capi):
         capi.preference_loss(loss, rewards, logp, saved, dlogp, x, tokens, torch.tensor(offsets, device="cuda"), torch.zeros(2, device="cuda"))
         for row, count in zip(guard, (1, 2, 12, 12, 24)):
             assert bool((row[:16] == 7.0).all()) and bool((row[16 + count:] == 7.0).all())
+
+
+def test_kinds_beyond_32_bits(capi):
+    def full(*size, dtype=torch.float32):
+        return torch.zeros(*size, dtype=dtype, device="cuda")
+
+    for kind in (2, -1, 1 << 32, (1 << 32) + 1, -(1 << 32)):
+        with pytest.raises(capi.NnfError, match="kind"):
+            capi.preference_loss(full(1), full(2), full(4), full(2, 4), full(4), full(4, 10), full(4, dtype=torch.int64), full(3, dtype=torch.int64), full(2), kind=kind)
